@@ -84,7 +84,7 @@ def draw(rng):
     Hkv, G, D = rng.choice([1, 2, 4, 8]), rng.choice([1, 1, 2, 3, 4, 8]), rng.choice([16, 24, 32, 40, 64, 80, 96, 128])
     if kind == "cache":
         B, Lk, Lq = _log_int(rng, 1, 32), _log_int(rng, 1, 32768), rng.choice([1, 1, 1, 2, 4, 7])
-        Lk = max(Lq, min(Lk, 130_000_000 // (B * Hkv * D)))
+        Lk = max(Lq, min(Lk, (130_000_000 if dtype == "bf16" else 65_000_000) // (B * Hkv * D)))
         return _attn(None, "forward", dtype, B, Lq, Lk, Hkv * G, Hkv, D, rng.random() < 0.5, rng.random() < 0.7, rng.random() < 0.2)
     B, Lk = _log_int(rng, 1, 16), _log_int(rng, 16, 8192)
     most = (4.5e11 if dtype == "bf16" else 4.5e10) / ((14 if kind == "step" else 4) * D * Hkv * G)  # pairs of one head
