@@ -82,6 +82,18 @@ class SemArgs(C.Structure):
                 ("ray_row_width", C.c_int), ("ray_row_offset", C.c_int)]
 
 
+class AttnArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("B", C.c_int), ("Lq", C.c_int), ("Lk", C.c_int), ("Hq", C.c_int),
+                ("Hkv", C.c_int), ("D", C.c_int), ("causal", C.c_int), ("scale", C.c_float),
+                ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("q_stride", C.c_longlong * 3), ("k_stride", C.c_longlong * 3), ("v_stride", C.c_longlong * 3),
+                ("lengths", C.c_void_p), ("key_mask", C.c_void_p), ("key_mask_stride", C.c_longlong),
+                ("q_start", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+                ("dout", C.c_void_p), ("dout_stride", C.c_longlong * 3),
+                ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 _P = C.c_void_p
 _SIGS = {
     "gpn_abi_version": (C.c_int, []),
@@ -121,6 +133,9 @@ _SIGS = {
                                   C.POINTER(SemArgs), _P, _P, _P, _P, C.c_size_t, _P]),
     "gpn_gnt_forward_static": (C.c_int, [C.POINTER(GntWeights), _P, C.c_int, _P, _P, _P, _P, _P, C.c_int,
                                          C.c_int, C.c_int, C.POINTER(SemArgs), _P, _P, _P, _P]),
+    "gpn_attn_workspace_bytes": (C.c_size_t, [C.POINTER(AttnArgs), C.c_int]),
+    "gpn_attn_forward": (C.c_int, [C.POINTER(AttnArgs), _P]),
+    "gpn_attn_backward": (C.c_int, [C.POINTER(AttnArgs), _P]),
     "gpn_timing_begin": (C.c_int, [C.c_uint, C.c_int]),
     "gpn_timing_end": (C.c_int, [C.POINTER(C.c_double), C.POINTER(C.c_longlong)]),
 }
@@ -207,6 +222,29 @@ class stage_timing:
         self.ms = {s: ms[i] for i, s in enumerate(STAGES)}
         self.launches = {s: cnt[i] for i, s in enumerate(STAGES)}
         return False
+
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1}  # GPN_DT_* of include/gpnerf_hip.h
+
+
+def dev_float(t, name, shape=None, dtype=None):
+    """Like dev_f32 for the operators that take float32 or bfloat16 and any strides."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s: expected a torch.Tensor" % name)
+    if not t.is_cuda:
+        raise RuntimeError("%s: tensor is on %s; gp-nerf_amd runs on HIP devices only (no CPU "
+                           "fallback)" % (name, t.device))
+    if t.dtype not in DTYPES or (dtype is not None and t.dtype != dtype):
+        raise ValueError("%s: expected %s, got %s" % (name, dtype or "float32 or bfloat16", t.dtype))
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError("%s: expected shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    return t
+
+
+def same_device(first, **others):
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError("%s: tensor is on %s, the first argument on %s" % (name, t.device, first.device))
 
 
 PRECISIONS = {"fp32": 0, "bf16x3": 1, "bf16": 2}  # GPN_PREC_* of include/gpnerf_hip.h

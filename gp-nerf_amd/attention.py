@@ -1,0 +1,164 @@
+"""Softmax attention with its gradients, on the HIP kernels of csrc/attention.hip (`gpn_attn_forward`, `gpn_attn_backward`).
+
+The renderer's own ray attention (`gpn_ray_attn`) is one fused, inference-only launch for rays of at most 128 samples.  The
+functions here are its inner product (reference gpnerf/transformer_network.py:155-178, attn_mode 'qk') for what that launch does
+not cover: training, longer sequences, masks, shared key/value heads, and single queries against a cache.
+
+    out, lse = attention_forward(q, k, v)                     no graph: inference, captured loops, hand-written steps
+    dq, dk, dv = attention_backward(dout, q, k, v, out, lse)
+    out = attention(q, k, v)                                  the same pair behind torch.autograd
+
+q is [B, Lq, Hq, D]; k and v are [B, Lk, Hkv, D]; query head h reads key/value head h // (Hq // Hkv).  float32 or bfloat16, all
+of one type; D a multiple of 8 up to 128.  Any strides (slices of a cache, expanded tensors); a tensor whose last dimension is
+not contiguous or whose rows are not 16-byte aligned is copied first.
+
+A key is visible to a query where all of these hold:
+    lengths   [B] int32: the key's position is below its batch's length
+    key_mask  [B, Lk] bool or uint8: its entry is not zero
+    causal    its position is at most q_start[b] + i for query i.  q_start [B] int32; without it queries are the last
+              Lq of Lk positions (Lk - Lq).  For a cache that is filled to `lengths`, q_start = lengths - Lq.
+A query that sees no key has out = 0, lse = -inf and no gradient.  Keys hidden by lengths or key_mask are never read: padding
+may hold anything.  Keys hidden by causal alone have to be finite, and so have the padding rows of q and dout.
+"""
+import ctypes as C
+import math
+
+import torch
+
+from . import _lib
+
+MAX_D = 128
+
+
+def _rows(t):
+    """(tensor the kernels can read, its strides between batches, positions and heads): 16-byte rows, contiguous along D."""
+    per = 16 // t.element_size()
+    for copy in (None, torch.Tensor.contiguous, torch.Tensor.clone):
+        if copy is not None:
+            t = copy(t)
+        s = t.stride()
+        n = t.shape
+        st = (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+        if s[3] == 1 and t.data_ptr() % 16 == 0 and not (st[0] % per or st[1] % per or st[2] % per):
+            return t, st
+    raise AssertionError("unreachable: a clone is aligned")
+
+
+def _index(t, name, B, dev):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != (B,) or t.device != dev:
+        raise ValueError("%s: expected an int32 tensor of shape (%d,) on %s" % (name, B, dev))
+    return t.contiguous()
+
+
+def _args(q, k, v, lengths, key_mask, causal, q_start, scale):
+    """Checks what both directions take -> (gpn_attn_args_t without outputs, tensors that have to live until the launch)."""
+    _lib.dev_float(q, "q")
+    _lib.dev_float(k, "k", dtype=q.dtype)
+    _lib.dev_float(v, "v", dtype=q.dtype)
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("q must be [B, Lq, Hq, D] and k [B, Lk, Hkv, D]")
+    B, Lq, Hq, D = q.shape
+    Lk, Hkv = k.shape[1], k.shape[2]
+    if k.shape[0] != B or k.shape[3] != D or v.shape != k.shape:
+        raise ValueError("k and v must be [%d, Lk, Hkv, %d] (got %s and %s)" % (B, D, tuple(k.shape), tuple(v.shape)))
+    if D % 8 or not 8 <= D <= MAX_D:
+        raise ValueError("head width must be a multiple of 8 up to %d (got %d)" % (MAX_D, D))
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError("%d query heads cannot share %d key/value heads" % (Hq, Hkv))
+    _lib.same_device(q, k=k, v=v)
+    if q_start is not None and not causal:
+        raise ValueError("q_start: only causal attention has positions")
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    q, sq = _rows(q)
+    k, sk = _rows(k)
+    v, sv = _rows(v)
+    a = _lib.AttnArgs(_lib.DTYPES[q.dtype], B, Lq, Lk, Hq, Hkv, D, 1 if causal else 0, scale, q.data_ptr(), k.data_ptr(),
+                      v.data_ptr(), sq, sk, sv)
+    keep = [q, k, v]
+    if lengths is not None:
+        lengths = _index(lengths, "lengths", B, q.device)
+        a.lengths = lengths.data_ptr()
+        keep.append(lengths)
+    if q_start is not None:
+        q_start = _index(q_start, "q_start", B, q.device)
+        a.q_start = q_start.data_ptr()
+        keep.append(q_start)
+    if key_mask is not None:
+        if not isinstance(key_mask, torch.Tensor) or key_mask.dtype not in (torch.bool, torch.uint8) or \
+                tuple(key_mask.shape) != (B, Lk) or key_mask.device != q.device:
+            raise ValueError("key_mask: expected a bool or uint8 tensor of shape (%d, %d) on %s" % (B, Lk, q.device))
+        if Lk > 1 and key_mask.stride(1) != 1:
+            key_mask = key_mask.contiguous()
+        a.key_mask, a.key_mask_stride = key_mask.data_ptr(), key_mask.stride(0)
+        keep.append(key_mask)
+    return a, keep
+
+
+def _call(a, backward, dev):
+    """Workspace and launch on the current stream of the tensors' device."""
+    L = _lib.lib()
+    with torch.cuda.device(dev):
+        need = L.gpn_attn_workspace_bytes(C.byref(a), backward)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        if need:
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need
+        fn, name = (L.gpn_attn_backward, "gpn_attn_backward") if backward else (L.gpn_attn_forward, "gpn_attn_forward")
+        _lib.check(fn(C.byref(a), _lib.stream()), name)
+
+
+@torch.no_grad()
+def attention_forward(q, k, v, lengths=None, key_mask=None, causal=False, q_start=None, scale=None):
+    """-> out [B, Lq, Hq, D] of q's type, lse [B, Hq, Lq] float32 (natural logarithm of the row's sum; -inf without a key).
+    scale: of the scores, positive (1 / sqrt(D) unless given)."""
+    a, keep = _args(q, k, v, lengths, key_mask, causal, q_start, scale)
+    B, Lq, Hq, D = q.shape
+    out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device)
+    a.out, a.lse = out.data_ptr(), lse.data_ptr()
+    _call(a, 0, q.device)
+    return out, lse
+
+
+@torch.no_grad()
+def attention_backward(dout, q, k, v, out, lse, lengths=None, key_mask=None, causal=False, q_start=None, scale=None):
+    """Gradients of sum(out * dout) -> dq, dk, dv (shapes and type of q, k, v, contiguous).  out and lse are what
+    attention_forward returned for the same arguments; the probabilities are computed again from them."""
+    a, keep = _args(q, k, v, lengths, key_mask, causal, q_start, scale)
+    B, Lq, Hq, D = q.shape
+    _lib.dev_float(dout, "dout", (B, Lq, Hq, D), q.dtype)
+    _lib.dev_float(out, "out", (B, Lq, Hq, D), q.dtype)
+    _lib.dev_float(lse, "lse", (B, Hq, Lq), torch.float32)
+    _lib.same_device(q, dout=dout, out=out, lse=lse)
+    dout, sdo = _rows(dout)
+    out = out if out.is_contiguous() and out.data_ptr() % 16 == 0 else out.clone(memory_format=torch.contiguous_format)
+    lse = lse.contiguous()
+    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
+    a.out, a.lse, a.dout, a.dout_stride = out.data_ptr(), lse.data_ptr(), dout.data_ptr(), sdo
+    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    _call(a, 1, q.device)
+    return dq, dk, dv
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, key_mask, causal, q_start, scale):
+        if any(ctx.needs_input_grad) and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("attention: a graph that autograd records cannot be captured safely (its leaves may belong to an "
+                               "eager graph on another stream); capture attention_forward and attention_backward instead")
+        out, lse = attention_forward(q, k, v, lengths, key_mask, causal, q_start, scale)
+        ctx.save_for_backward(q, k, v, out, lse, lengths, key_mask, q_start)
+        ctx.causal, ctx.scale = causal, scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, lengths, key_mask, q_start = ctx.saved_tensors
+        grads = attention_backward(dout, q, k, v, out, lse, lengths, key_mask, ctx.causal, q_start, ctx.scale)
+        return (*grads, None, None, None, None, None)
+
+
+def attention(q, k, v, lengths=None, key_mask=None, causal=False, q_start=None, scale=None):
+    """attention_forward's output, differentiable in q, k and v (once; not inside a captured graph)."""
+    return _Attention.apply(q, k, v, lengths, key_mask, causal, q_start, scale)

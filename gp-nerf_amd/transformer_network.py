@@ -2,15 +2,20 @@
 signature as reference gpnerf/transformer_network.py:221-338; the forward pass runs entirely in the
 fp32-MFMA HIP kernels of csrc/gnt.hip through `gpn_gnt_forward`.
 
-Inference only (eval-mode semantics: the reference's Dropout(0.1) layers are identities in eval,
-reference eval_gpnerf.py:172); no autograd graph is built.
+`GNT.forward` is inference only (eval-mode semantics: the reference's Dropout(0.1) layers are identities in eval,
+reference eval_gpnerf.py:172); no autograd graph is built.  The ray attention of a block can be trained by itself:
+`net.view_selftrans[i].attn(x)` runs on the differentiable kernels of `attention.attention`.
 """
 import ctypes as C
 
 import torch
 import torch.nn as nn
+from torch.nn import functional as F
 
 from . import _lib
+from .attention import attention
+
+RAY_HEADS = 4  # heads of the ray attention (reference :131)
 
 
 class _Lin(nn.Module):
@@ -70,6 +75,14 @@ class _RayAttn(nn.Module):  # Attention, attn_mode='qk' (reference :130-147)
         self.k_fc = _Lin(dim, dim, bias=False)
         self.v_fc = _Lin(dim, dim, bias=False)
         self.out_fc = _Lin(dim, dim)
+
+    def forward(self, x, key_mask=None):
+        """reference :149-178 (without its Dropout), differentiable: x [R, S, C] -> [R, S, C], any S, float32 or (module and
+        x) bfloat16.  key_mask [R, S]: samples that no other sample attends to (e.g. those that no view sees).  The renderer
+        does not come here: its layers run in gpn_ray_attn."""
+        R, S, dim = x.shape
+        q, k, v = (F.linear(x, fc.weight).view(R, S, RAY_HEADS, dim // RAY_HEADS) for fc in (self.q_fc, self.k_fc, self.v_fc))
+        return F.linear(attention(q, k, v, key_mask=key_mask).view(R, S, dim), self.out_fc.weight, self.out_fc.bias)
 
 
 class _Block(nn.Module):  # Transformer2D / Transformer (reference :97-104, :191-200)

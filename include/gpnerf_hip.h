@@ -378,6 +378,50 @@ int gpn_gnt_forward_static(const gpn_gnt_weights_t* W, const float* rgb_feat, in
                            gpn_sem_args_t* sem, float* out, float* depth, float* sem_feat,
                            gpn_stream_t stream);
 
+/* ------------------------------------------------------------------ softmax attention with its gradients
+ * The training counterpart of the ray attention's inner product (reference transformer_network.py:155-178, Attention with
+ * attn_mode 'qk', between its linear layers), for any lengths and head layout; no length limit of gpn_ray_attn applies.
+ *
+ *   visible(b,i,j) = j < lengths[b]  and  key_mask[b][j] != 0  and  (not causal or j <= q_start[b] + i)
+ *   s = scale q_i . k_j;  lse_i = log sum_visible exp(s);  out_i = sum_visible exp(s - lse_i) v_j
+ *
+ * Query head h reads key/value head h / (Hq / Hkv).  A row that sees no key has out = 0, lse = -inf and zero gradients.
+ * Keys that lengths or key_mask hide are never read (they may hold NaN); dk and dv are written for all Lk keys, zero for hidden
+ * ones.  Keys hidden from a row by `causal` alone are read for it and must be finite, as must q and dout rows that are padding.
+ * lengths are taken into [0, Lk]; q_start may be negative.  Sums, maxima and exponentials are fp32; in bf16 the
+ * probabilities and their gradients are rounded to bf16 (half a step, 2^-8) as operands of the second products.
+ * Results do not depend on the order in which workgroups run: there is no atomic. */
+#define GPN_DT_F32 0
+#define GPN_DT_BF16 1
+#define GPN_ATTN_MAX_D 128
+
+typedef struct {
+  int dtype;                 /* GPN_DT_*: of q, k, v, out, dout, dq, dk, dv */
+  int B, Lq, Lk, Hq, Hkv, D; /* Hq a multiple of Hkv; D a multiple of 8, at most GPN_ATTN_MAX_D */
+  int causal;
+  float scale;               /* positive, finite */
+  const void *q, *k, *v;     /* [B,Lq,Hq,D], [B,Lk,Hkv,D] x 2: 16-byte aligned, contiguous along D, and strided: */
+  long long q_stride[3], k_stride[3], v_stride[3]; /* elements between batches, positions, heads (multiples of 16 bytes; 0 is
+                                                      a broadcast) */
+  const int32_t* lengths;    /* [B] number of keys of each batch, or NULL: Lk */
+  const uint8_t* key_mask;   /* [B,Lk] 0 = hidden, or NULL */
+  long long key_mask_stride; /* bytes between its rows */
+  const int32_t* q_start;    /* [B] position of query 0 among the keys (causal only), or NULL: Lk - Lq */
+  void* out;                 /* [B,Lq,Hq,D] contiguous: written by the forward, read by the backward */
+  float* lse;                /* [B,Hq,Lq]: likewise (natural logarithm) */
+  const void* dout;          /* backward: [B,Lq,Hq,D], strided like q */
+  long long dout_stride[3];
+  void *dq, *dk, *dv;        /* backward, out: shapes of q, k, v, contiguous */
+  void* workspace;           /* gpn_attn_workspace_bytes(args, backward) bytes of device memory, 256-byte aligned */
+  size_t workspace_bytes;
+} gpn_attn_args_t;
+
+/* Depends on the sizes alone; 0 for sizes that gpn_attn_forward / gpn_attn_backward refuse. */
+size_t gpn_attn_workspace_bytes(const gpn_attn_args_t* a, int backward);
+int gpn_attn_forward(const gpn_attn_args_t* a, gpn_stream_t stream);
+/* dq, dk, dv of sum(out * dout): the probabilities are computed again from q, k and lse. */
+int gpn_attn_backward(const gpn_attn_args_t* a, gpn_stream_t stream);
+
 /* ------------------------------------------------------------------ measurement hooks
  * No counterpart in the reference: bench.py uses these to time individual kernels with HIP events on
  * the stream they are launched on, inside the timed region.  gpn_timing_begin creates `max_records`
