@@ -94,6 +94,16 @@ class AttnArgs(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class DistillArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("teacher_dtype", C.c_int), ("index_bytes", C.c_int), ("C", C.c_int),
+                ("K", C.c_int), ("reduction", C.c_int), ("temperature", C.c_float), ("grad_scale", C.c_float),
+                ("N", C.c_longlong), ("logits", C.c_void_p), ("row_stride", C.c_longlong),
+                ("class_stride", C.c_longlong), ("teacher", C.c_void_p), ("teacher_stride", C.c_longlong * 2),
+                ("index", C.c_void_p), ("index_stride", C.c_longlong * 2), ("row_weight", C.c_void_p),
+                ("loss_rows", C.c_void_p), ("loss", C.c_void_p), ("lse", C.c_void_p), ("dloss", C.c_void_p),
+                ("dlogits", C.c_void_p), ("drow_stride", C.c_longlong), ("dclass_stride", C.c_longlong)]
+
+
 _P = C.c_void_p
 _SIGS = {
     "gpn_abi_version": (C.c_int, []),
@@ -136,6 +146,9 @@ _SIGS = {
     "gpn_attn_workspace_bytes": (C.c_size_t, [C.POINTER(AttnArgs), C.c_int]),
     "gpn_attn_forward": (C.c_int, [C.POINTER(AttnArgs), _P]),
     "gpn_attn_backward": (C.c_int, [C.POINTER(AttnArgs), _P]),
+    "gpn_distill_forward": (C.c_int, [C.POINTER(DistillArgs), _P]),
+    "gpn_distill_backward": (C.c_int, [C.POINTER(DistillArgs), _P]),
+    "gpn_distill_step": (C.c_int, [C.POINTER(DistillArgs), _P]),
     "gpn_timing_begin": (C.c_int, [C.c_uint, C.c_int]),
     "gpn_timing_end": (C.c_int, [C.POINTER(C.c_double), C.POINTER(C.c_longlong)]),
 }

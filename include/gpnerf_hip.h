@@ -422,6 +422,49 @@ int gpn_attn_forward(const gpn_attn_args_t* a, gpn_stream_t stream);
 /* dq, dk, dv of sum(out * dout): the probabilities are computed again from q, k and lse. */
 int gpn_attn_backward(const gpn_attn_args_t* a, gpn_stream_t stream);
 
+/* ------------------------------------------------------------------ distillation from a teacher's top logits
+ * The loss that class logits learn from a 2-D teacher by (the training branch of the semantic head, reference
+ * semantic_branch.py:60-88, here against the teacher's K largest logits of every row instead of its features):
+ *
+ *   p = softmax_k(t_k / T);   ls_c = z_c / T - log sum_c' exp(z_c' / T)
+ *   loss_n = T^2 w_n sum_k p_k (log p_k - ls_{index_k});     dz_c = g_n w_n T (exp(ls_c) - sum_{k: index_k = c} p_k)
+ *
+ * An entry whose index is outside [0, C) is left out; a row without an entry (or whose entries are all -inf) has loss 0 and
+ * gradient 0 whatever its logits hold.  The same class twice in a row counts twice.  The teacher takes no gradient.
+ * dlogits may not overlap the logits.  N = 0 is a loss of 0. */
+#define GPN_DISTILL_MAX_K 256
+#define GPN_RED_NONE 0
+#define GPN_RED_SUM 1
+#define GPN_RED_MEAN 2 /* over all N rows */
+
+typedef struct {
+  int dtype, teacher_dtype;   /* GPN_DT_* of logits and dlogits / of teacher */
+  int index_bytes;            /* 4 or 8: index is int32 or int64 */
+  int C, K;
+  int reduction;              /* GPN_RED_* */
+  float temperature;
+  float grad_scale;           /* gpn_distill_step: dlogits is the gradient of grad_scale * loss */
+  long long N;
+  const void* logits;         /* element (n, c) at n * row_stride + c * class_stride; one of the two strides is 1 */
+  long long row_stride, class_stride;
+  const void* teacher;        /* [N,K] with any strides */
+  long long teacher_stride[2];
+  const void* index;          /* [N,K] with any strides */
+  long long index_stride[2];
+  const float* row_weight;    /* [N] or NULL: 1 */
+  float* loss_rows;           /* [N], written by forward and step */
+  float* loss;                /* [1]: their sum or mean (reduction other than none) */
+  float* lse;                 /* [N], written by forward, read by backward: log sum exp(z / T) */
+  const float* dloss;         /* backward: [N] for GPN_RED_NONE, else [1] */
+  void* dlogits;              /* laid out as the logits are (contiguous classes, or contiguous rows) */
+  long long drow_stride, dclass_stride;
+} gpn_distill_args_t;
+
+int gpn_distill_forward(const gpn_distill_args_t* a, gpn_stream_t stream);
+int gpn_distill_backward(const gpn_distill_args_t* a, gpn_stream_t stream);
+/* Forward and backward in one pass, for a loss whose upstream gradient is known beforehand: the logits are read once. */
+int gpn_distill_step(const gpn_distill_args_t* a, gpn_stream_t stream);
+
 /* ------------------------------------------------------------------ measurement hooks
  * No counterpart in the reference: bench.py uses these to time individual kernels with HIP events on
  * the stream they are launched on, inside the timed region.  gpn_timing_begin creates `max_records`
