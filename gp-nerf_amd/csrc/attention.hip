@@ -256,7 +256,7 @@ struct Fwd {
 extern __shared__ __attribute__((aligned(16))) unsigned char attn_smem[];
 
 template <typename T, int DP, int WM, int WK, int KT, int NBUF>
-__global__ void __launch_bounds__(64 * WM * WK) k_attn_fwd(const AttnP a) {
+__global__ void __launch_bounds__(64 * WM * WK, 2) k_attn_fwd(const AttnP a) {
   using F = Fwd<T, DP, WM, WK, KT, NBUF>;
   using M = Mt<T>;
   constexpr int TM = F::TM, MT = F::MT, BN = F::BN, BM = F::BM, NTH = F::NTH, KF = F::KF, MD = F::MD, LK = F::LK, LV = F::LV;
@@ -345,10 +345,18 @@ __global__ void __launch_bounds__(64 * WM * WK) k_attn_fwd(const AttnP a) {
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int r = 0; r < M::NC; ++r) mx = fmaxf(mx, sc[mt][r]);
-      mx = fmaxf(m, col_max<T>(mx));
-      const float mc = mx == -INFINITY ? 0.f : mx * a.c;  // a row that has seen nothing yet
-      const float alpha = exp2_(m * a.c - mc);
-      m = mx;
+      // The row's reference moves only when a score exceeds it by 8 powers of two: until then the sums just grow, in fp32, and
+      // the products' operands keep their relative precision.  alpha is 1 for the rows of the wave that stay.
+      mx = col_max<T>(mx);
+      const bool grow = (mx - m) * a.c > 8.f;  // of a row without a key so far: inf > 8; still without: nan > 8
+      if (__any(grow)) {
+        const float alpha = grow ? exp2_((m - mx) * a.c) : 1.f;
+        m = grow ? mx : m;
+        l *= alpha;
+#pragma unroll
+        for (int md = 0; md < MD; ++md) o[md] *= alpha;
+      }
+      const float mc = m == -INFINITY ? 0.f : m * a.c;
       float sum = 0.f;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
@@ -358,9 +366,7 @@ __global__ void __launch_bounds__(64 * WM * WK) k_attn_fwd(const AttnP a) {
           sc[mt][r] = e;
           sum += e;
         }
-      l = l * alpha + sum;
-#pragma unroll
-      for (int md = 0; md < MD; ++md) o[md] *= alpha;
+      l += sum;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -482,7 +488,7 @@ struct Dq {
 };
 
 template <typename T, int DP, int WM, int KT>
-__global__ void __launch_bounds__(64 * WM) k_attn_dq(const AttnP a) {
+__global__ void __launch_bounds__(64 * WM, 2) k_attn_dq(const AttnP a) {
   using F = Dq<T, DP, WM, KT>;
   using M = Mt<T>;
   constexpr int TM = F::TM, MT = F::MT, BM = F::BM, NTH = F::NTH, KF = F::KF, MD = F::MD, LK = F::LK, LV = F::LV;
@@ -581,41 +587,42 @@ __global__ void __launch_bounds__(64 * WM) k_attn_dq(const AttnP a) {
 
 // ---------------------------------------------------------------------------------------------- gradients of keys, values
 // Keys and values are stationary, a wave holds TM of them; the rows of all query heads that share them walk past, so the sum
-// over the group is part of the walk and its order is fixed.
-template <typename T, int DP, int W, int RB>
+// over the group is part of the walk and its order is fixed.  WN waves along the keys x WR waves along the rows: the WR waves of
+// the same keys take the rows of a stage in turns and join their sums at the end, so that two waves fit a SIMD (256 registers)
+// without a second copy of the keys' sums in memory.  Where those registers are short (VL) the values come from LDS.
+// Work is cut evenly: under `causal` a workgroup takes the key tiles t and tiles - 1 - t, which together see as many rows as any
+// other such pair, and every tile's own rows are cut into nsplit parts (fp32 sums in the workspace, joined in order).
+template <typename T, int DP, int WN, int WR>
 struct Dkv {
   using M = Mt<T>;
-  static constexpr int TM = M::TM, MT = RB / TM, BN = W * TM, NTH = 64 * W, KF = DP / 16;
-  static constexpr int DV = Ld<T, DP>::DV, MD = DV / TM, LQ = Ld<T, DP>::both;
-  static constexpr size_t lds = (size_t)2 * (2 * RB * LQ * sizeof(T) + 2 * RB * 4);
+  static constexpr int TM = M::TM, RW = sizeof(T) == 4 && DP > 64 ? 16 : 32, RB = WR * RW, MT = RW / TM, BN = WN * TM, NTH = 64 * WN * WR, KF = DP / 16;
+  static constexpr int DV = Ld<T, DP>::DV, MD = DV / TM, LQ = Ld<T, DP>::both, LV = Ld<T, DP>::row;
+  static constexpr bool VL = DP > 64;
+  static constexpr size_t stage_bytes = (size_t)2 * (2 * RB * LQ * sizeof(T) + 2 * RB * 4) + (VL ? BN * LV * sizeof(T) : 0);
+  static constexpr size_t join_bytes = WR > 1 ? (size_t)WN * 2 * MD * M::NC * 64 * 4 : 0;
+  static constexpr size_t lds = stage_bytes > join_bytes ? stage_bytes : join_bytes;
 };
 
-template <typename T, int DP, int W, int RB>
-__global__ void __launch_bounds__(64 * W) k_attn_dkv(const AttnP a) {
-  using F = Dkv<T, DP, W, RB>;
+template <typename T, int DP, int WN, int WR>
+__global__ void __launch_bounds__(64 * WN * WR, 2) k_attn_dkv(const AttnP a) {
+  using F = Dkv<T, DP, WN, WR>;
   using M = Mt<T>;
-  constexpr int TM = F::TM, MT = F::MT, BN = F::BN, NTH = F::NTH, KF = F::KF, MD = F::MD, LQ = F::LQ;
-  int pr, tile;
-  if (!locate(a.B * a.Hkv, a.tiles, pr, tile)) return;
+  static_assert(WR == 1 || WR == 2, "the join below exchanges between two waves");
+  constexpr int TM = F::TM, MT = F::MT, RB = F::RB, BN = F::BN, NTH = F::NTH, KF = F::KF, MD = F::MD, LQ = F::LQ, LV = F::LV;
+  constexpr bool VL = F::VL;
+  int pr, unit;
+  if (!locate(a.B * a.Hkv, (a.causal ? (a.tiles + 1) / 2 : a.tiles) * a.nsplit, pr, unit)) return;
+  const int tu = unit / a.nsplit, split = unit - tu * a.nsplit;
   const Prob p = problem(a, pr);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave % WN, wr = wave / WN;
   const int n = lane & (TM - 1), h = lane / TM;
-  const int j0 = tile * BN, key = j0 + wave * TM + n;
   const unsigned char* km = a.key_mask ? a.key_mask + p.b * a.mask_sb : nullptr;
-  const bool seen = key < p.len && (!km || km[key]);
-  // first row that sees the lane's key / any key of the workgroup / whole tile of the wave
   const auto first_row = [&](int j) { return !a.causal || j <= p.qs ? 0 : j - p.qs >= a.Lq ? INT_MAX : (j - p.qs) * a.G; };
-  const int rmin = first_row(key), rall = first_row(j0 + wave * TM + TM - 1);
-  int rbeg = j0 < p.len ? first_row(j0) : INT_MAX;
-  rbeg = rbeg < a.M ? rbeg - rbeg % RB : a.M;
 
-  typename M::Frag kf[KF], vf[KF];
-  load_frags<T, KF>(kf, seen ? (const T*)a.k + p.b * a.sk.b + key * a.sk.l + p.hk * a.sk.h : nullptr, a.D, h);
-  load_frags<T, KF>(vf, seen ? (const T*)a.v + p.b * a.sv.b + key * a.sv.l + p.hk * a.sv.h : nullptr, a.D, h);
-
-  T* qs = (T*)attn_smem;       // [2][RB][LQ]
-  T* ds = qs + 2 * RB * LQ;    // [2][RB][LQ]
+  T* qs = (T*)attn_smem;                   // [2][RB][LQ]
+  T* ds = qs + 2 * RB * LQ;                // [2][RB][LQ]
   float* ls = (float*)(ds + 2 * RB * LQ);  // [2][RB] log-sum-exp (log2), [2][RB] delta
+  T* vs = (T*)(ls + 4 * RB);               // [BN][LV]
   Stage<T, DP, RB, NTH> sq, sd;
   float rl, rd;
   const auto request = [&](int r0) {
@@ -640,67 +647,152 @@ __global__ void __launch_bounds__(64 * W) k_attn_dkv(const AttnP a) {
     sq.store(qs + buf * RB * LQ, LQ), sd.store(ds + buf * RB * LQ, LQ);
     if (threadIdx.x < RB) ls[buf * RB + threadIdx.x] = rl, ls[(2 + buf) * RB + threadIdx.x] = rd;
   };
-  typename M::Acc dk[MD], dv[MD];
-#pragma unroll
-  for (int md = 0; md < MD; ++md) dk[md] = dv[md] = (typename M::Acc)(0.f);
-  if (rbeg < a.M) {
-    request(rbeg);
-    put(0);
-    if (rbeg + RB < a.M) request(rbeg + RB);
-    __syncthreads();
-  }
-  int buf = 0;
-  for (int r0 = rbeg; r0 < a.M; r0 += RB, buf ^= 1) {
-    if (r0 + RB < a.M) {
-      put(buf ^ 1);
-      if (r0 + 2 * RB < a.M) request(r0 + 2 * RB);
+
+  for (int half = 0; half < (a.causal ? 2 : 1); ++half) {
+    const int tile = half ? a.tiles - 1 - tu : tu;
+    if (half && tile <= tu) break;
+    if (half) __syncthreads();  // the join of the first tile has been read
+    const int j0 = tile * BN, key = j0 + wn * TM + n;
+    const bool seen = key < p.len && (!km || km[key]);
+    // first row that sees the lane's key / the wave's first key / all of the wave's keys
+    const int rmin = first_row(key), rany = first_row(j0 + wn * TM), rall = first_row(j0 + wn * TM + TM - 1);
+    int rbeg = j0 < p.len ? first_row(j0) : INT_MAX, rend = rbeg;
+    if (rbeg < a.M) {
+      const int b0 = rbeg / RB, blocks = (a.M + RB - 1) / RB - b0;
+      rbeg = (b0 + (int)((long long)blocks * split / a.nsplit)) * RB;
+      rend = min((b0 + (int)((long long)blocks * (split + 1) / a.nsplit)) * RB, a.M);
     }
-    if (r0 + RB > first_row(j0 + wave * TM)) {
-      const bool partly = r0 < rall;
+
+    typename M::Frag kf[KF], vf[VL ? 1 : KF];
+    load_frags<T, KF>(kf, seen ? (const T*)a.k + p.b * a.sk.b + key * a.sk.l + p.hk * a.sk.h : nullptr, a.D, h);
+    if constexpr (VL) {
+      Stage<T, DP, BN, NTH> sv;
+      sv.load(a.D, [&](int j) {
+        return j0 + j < p.len && (!km || km[j0 + j]) ? (const T*)a.v + p.b * a.sv.b + (j0 + j) * a.sv.l + p.hk * a.sv.h
+                                                     : (const T*)nullptr;
+      });
+      sv.store(vs, LV);
+    } else {
+      load_frags<T, KF>(vf, seen ? (const T*)a.v + p.b * a.sv.b + key * a.sv.l + p.hk * a.sv.h : nullptr, a.D, h);
+    }
+    const T* vw = vs + wn * TM * LV;
+
+    typename M::Acc dk[MD], dv[MD];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const T* qt = qs + (buf * RB + mt * TM) * LQ;
-        const T* dt = ds + (buf * RB + mt * TM) * LQ;
-        typename M::Acc sc = (typename M::Acc)(0.f), dp = (typename M::Acc)(0.f);
+    for (int md = 0; md < MD; ++md) dk[md] = dv[md] = (typename M::Acc)(0.f);
+    if (rbeg < rend) {
+      request(rbeg);
+      put(0);
+      if (rbeg + RB < rend) request(rbeg + RB);
+      __syncthreads();
+    }
+    int buf = 0;
+    for (int r0 = rbeg; r0 < rend; r0 += RB, buf ^= 1) {
+      if (r0 + RB < rend) {
+        put(buf ^ 1);
+        if (r0 + 2 * RB < rend) request(r0 + 2 * RB);
+      }
+      const int rw = r0 + wr * F::RW;
+      if (rw + F::RW > rany) {
+        const bool partly = rw < rall;
 #pragma unroll
-        for (int f = 0; f < KF; ++f) {
-          sc = M::mma(rowfrag<T>(qt + 16 * f, LQ, lane), kf[f], sc);
-          dp = M::mma(rowfrag<T>(dt + 16 * f, LQ, lane), vf[f], dp);
-        }
+        for (int mt = 0; mt < MT; ++mt) {
+          const int lr = buf * RB + wr * F::RW + mt * TM;  // the tile's row in LDS
+          const T* qt = qs + lr * LQ;
+          const T* dt = ds + lr * LQ;
+          typename M::Acc sc = (typename M::Acc)(0.f), dp = (typename M::Acc)(0.f);
 #pragma unroll
-        for (int q = 0; q < M::NC / 4; ++q) {
-          const int r = mt * TM + M::crow(4 * q, h);
-          const fl4 l4 = *(const fl4*)(ls + buf * RB + r), d4 = *(const fl4*)(ls + (2 + buf) * RB + r);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = exp2_(__builtin_fmaf(sc[4 * q + e], a.c, -l4[e]));
-            if (partly && r0 + r + e < rmin) x = 0.f;
-            sc[4 * q + e] = x;
-            dp[4 * q + e] = x * (dp[4 * q + e] - d4[e]);
+          for (int f = 0; f < KF; ++f) {
+            sc = M::mma(rowfrag<T>(qt + 16 * f, LQ, lane), kf[f], sc);
+            if constexpr (VL) dp = M::mma(rowfrag<T>(dt + 16 * f, LQ, lane), rowfrag<T>(vw + 16 * f, LV, lane), dp);
+            else dp = M::mma(rowfrag<T>(dt + 16 * f, LQ, lane), vf[f], dp);
           }
-        }
 #pragma unroll
-        for (int t = 0; t < TM / 16; ++t) {
-          const typename M::Frag pf = M::pack(sc, t), sf = M::pack(dp, t);
+          for (int q = 0; q < M::NC / 4; ++q) {
+            const int r = M::crow(4 * q, h);
+            const fl4 l4 = *(const fl4*)(ls + lr + r), d4 = *(const fl4*)(ls + 2 * RB + lr + r);
 #pragma unroll
-          for (int md = 0; md < MD; ++md) {
-            dv[md] = M::mma(M::colfrag(dt + 16 * t * LQ + md * TM, LQ, lane), pf, dv[md]);
-            dk[md] = M::mma(M::colfrag(qt + 16 * t * LQ + md * TM, LQ, lane), sf, dk[md]);
+            for (int e = 0; e < 4; ++e) {
+              float x = exp2_(__builtin_fmaf(sc[4 * q + e], a.c, -l4[e]));
+              if (partly && rw + mt * TM + r + e < rmin) x = 0.f;
+              sc[4 * q + e] = x;
+              dp[4 * q + e] = x * (dp[4 * q + e] - d4[e]);
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < TM / 16; ++t) {
+            const typename M::Frag pf = M::pack(sc, t), sf = M::pack(dp, t);
+#pragma unroll
+            for (int md = 0; md < MD; ++md) {
+              dv[md] = M::mma(M::colfrag(dt + 16 * t * LQ + md * TM, LQ, lane), pf, dv[md]);
+              dk[md] = M::mma(M::colfrag(qt + 16 * t * LQ + md * TM, LQ, lane), sf, dk[md]);
+            }
           }
         }
       }
+      __syncthreads();
     }
-    __syncthreads();
-  }
-  if (key < a.Lk) {
-    const long long at = (((long long)p.b * a.Lk + key) * a.Hkv + p.hk) * a.D;
-    if (!seen) {  // a hidden key's gradients are zero, whatever stood in its row
+    if constexpr (WR == 2) {  // wave 0 of a pair finishes dk, wave 1 finishes dv
+      fl4* x = (fl4*)attn_smem + (wn * 2) * MD * (M::NC / 4) * 64 + lane;
+      const auto give = [&](const typename M::Acc(&o)[MD], int slot) {
 #pragma unroll
-      for (int md = 0; md < MD; ++md) dk[md] = dv[md] = (typename M::Acc)(0.f);
+        for (int md = 0; md < MD; ++md)
+#pragma unroll
+          for (int q = 0; q < M::NC / 4; ++q) {
+            fl4 y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = o[md][4 * q + e];
+            x[((slot * MD + md) * (M::NC / 4) + q) * 64] = y;
+          }
+      };
+      const auto take = [&](typename M::Acc(&o)[MD], int slot) {
+#pragma unroll
+        for (int md = 0; md < MD; ++md)
+#pragma unroll
+          for (int q = 0; q < M::NC / 4; ++q) {
+            const fl4 y = x[((slot * MD + md) * (M::NC / 4) + q) * 64];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[md][4 * q + e] += y[e];
+          }
+      };
+      if (rbeg >= rend) __syncthreads();  // no stage: the values' tile may still be on its way into the same memory
+      if (wr) give(dk, 0);
+      else give(dv, 1);
+      __syncthreads();
+      if (wr) take(dv, 1);
+      else take(dk, 0);
     }
-    store_cols<T, T, MD>(dk, a.scale, (T*)a.dk + at, a.D, h);
-    store_cols<T, T, MD>(dv, 1.f, (T*)a.dv + at, a.D, h);
+    if (key < a.Lk) {
+      const long long at = (((long long)p.b * a.Lk + key) * a.Hkv + p.hk) * a.D;
+      const long long part = (long long)a.B * a.Lk * a.Hkv * a.D;
+      if (!seen) {  // a hidden key's gradients are zero, whatever stood in its row
+#pragma unroll
+        for (int md = 0; md < MD; ++md) dk[md] = dv[md] = (typename M::Acc)(0.f);
+      }
+      if (a.nsplit > 1) {
+        if (WR == 1 || !wr) store_cols<T, float, MD>(dk, a.scale, a.part_o + 2 * split * part + at, a.D, h);
+        if (WR == 1 || wr) store_cols<T, float, MD>(dv, 1.f, a.part_o + (2 * split + 1) * part + at, a.D, h);
+      } else {
+        if (WR == 1 || !wr) store_cols<T, T, MD>(dk, a.scale, (T*)a.dk + at, a.D, h);
+        if (WR == 1 || wr) store_cols<T, T, MD>(dv, 1.f, (T*)a.dv + at, a.D, h);
+      }
+    }
   }
+}
+
+// Sums the parts of dk and dv in order.  4 values a lane.
+template <typename T>
+__global__ void __launch_bounds__(256) k_attn_dkv_join(const AttnP a) {
+  const long long part = (long long)a.B * a.Lk * a.Hkv * a.D;
+  const long long x = 4 * ((long long)blockIdx.x * 256 + threadIdx.x);
+  if (x >= 2 * part) return;
+  fl4 s = (fl4)(0.f);
+  for (int i = 0; i < a.nsplit; ++i) s += *(const fl4*)(a.part_o + 2 * i * part + x);
+  typedef T V4 __attribute__((ext_vector_type(4)));
+  V4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = (T)s[e];
+  *(V4*)((T*)(x < part ? a.dk : a.dv) + (x < part ? x : x - part)) = y;
 }
 
 // ------------------------------------------------------------------------------------------------------------ host
@@ -811,8 +903,25 @@ int forward_t(AttnP& a, const Plan& pl, hipStream_t st) {
   return launch(k_attn_join<T>, "k_attn_join", (rows + 7) / 8, 256, 0, st, a);
 }
 
+// Keys of a workgroup of the dk / dv kernel: 4 waves' tiles.
+int dkv_keys(bool f32) { return f32 ? 64 : 128; }
+
+// Parts that the rows of a key tile are cut into: enough for two workgroups on every CU, with 256 rows or more each, so that a
+// part's products outweigh its sums' way through memory.
+int plan_dkv(const gpn_attn_args_t* x) {
+  const long long M = (long long)x->Lq * (x->Hq / x->Hkv);
+  const int bn = dkv_keys(x->dtype == GPN_DT_F32);
+  long long tiles = (x->Lk + bn - 1) / bn;
+  if (x->causal) tiles = (tiles + 1) / 2;
+  const long long units = (long long)x->B * x->Hkv * tiles;
+  if (units == 0 || units >= 256) return 1;
+  long long s = 512 / units;
+  if (s > M / 256) s = M / 256;
+  return s < 1 ? 1 : s > 16 ? 16 : (int)s;
+}
+
 template <typename T, int DP>
-int backward_t(AttnP& a, hipStream_t st) {
+int backward_t(AttnP& a, int nsplit, hipStream_t st) {
   constexpr bool F32 = sizeof(T) == 4;
   const long long prob = (long long)a.B * a.Hkv;
   {
@@ -822,9 +931,13 @@ int backward_t(AttnP& a, hipStream_t st) {
     const int rc = launch(k_attn_dq<T, DP, 4, KT>, "k_attn_dq", grid_of(prob, a.tiles), F::NTH, F::lds, st, a);
     if (rc) return rc;
   }
-  using F = Dkv<T, DP, 4, 32>;
-  a.tiles = (a.Lk + F::BN - 1) / F::BN;
-  return launch(k_attn_dkv<T, DP, 4, 32>, "k_attn_dkv", grid_of(prob, a.tiles), F::NTH, F::lds, st, a);
+  using F = Dkv<T, DP, 4, 2>;
+  static_assert(F::BN == (F32 ? 64 : 128) && F::lds <= 160 * 1024, "dkv_keys, LDS");
+  a.tiles = (a.Lk + F::BN - 1) / F::BN, a.nsplit = nsplit;
+  const long long units = (long long)(a.causal ? (a.tiles + 1) / 2 : a.tiles) * nsplit;
+  const int rc = launch(k_attn_dkv<T, DP, 4, 2>, "k_attn_dkv", grid_of(prob, units), F::NTH, F::lds, st, a);
+  if (rc || nsplit == 1) return rc;
+  return launch(k_attn_dkv_join<T>, "k_attn_dkv_join", ((long long)a.B * a.Lk * a.Hkv * a.D / 2 + 255) / 256, 256, 0, st, a);
 }
 
 template <typename Fn>
@@ -841,7 +954,10 @@ int by_width(int D, Fn fn) {  // head widths are padded to the next of these wit
 extern "C" size_t gpn_attn_workspace_bytes(const gpn_attn_args_t* x, int backward) {
   if (check_args(x, "gpn_attn_workspace_bytes") || x->B == 0 || x->Lq == 0) return 0;
   const size_t rows = (size_t)x->B * x->Hq * x->Lq;
-  if (backward) return align256(rows * 4);
+  if (backward) {  // delta, and the parts of dk and dv
+    const int s = plan_dkv(x);
+    return align256(rows * 4) + (s > 1 ? (size_t)s * 2 * x->B * x->Lk * x->Hkv * x->D * 4 : 0);
+  }
   const Plan p = plan_forward(x);
   return p.nsplit == 1 ? 0 : align256(rows * p.nsplit * 4) + rows * p.nsplit * x->D * 4;
 }
@@ -897,10 +1013,12 @@ extern "C" int gpn_attn_backward(const gpn_attn_args_t* x, gpn_stream_t stream) 
   GPN_REQUIRE(x->workspace_bytes >= need && (need == 0 || x->workspace), "%s: workspace of %zu bytes, %zu needed", name,
               x->workspace_bytes, need);
   AttnP a = fill(x);
+  const int nsplit = plan_dkv(x);
   a.delta = (float*)x->workspace;
+  a.part_o = (float*)((char*)x->workspace + align256((size_t)x->B * x->Hq * x->Lq * 4));
   hipStream_t st = (hipStream_t)stream;
   return by_width(x->D, [&](auto dp) {
-    return x->dtype == GPN_DT_F32 ? backward_t<float, decltype(dp)::value>(a, st)
-                                  : backward_t<bf16, decltype(dp)::value>(a, st);
+    return x->dtype == GPN_DT_F32 ? backward_t<float, decltype(dp)::value>(a, nsplit, st)
+                                  : backward_t<bf16, decltype(dp)::value>(a, nsplit, st);
   });
 }
