@@ -53,14 +53,6 @@ struct Mt<bf16> {  // v_mfma_f32_32x32x16_bf16
     for (int i = 0; i < 8; ++i) f[i] = (bf16)s[8 * t + i];
     return f;
   }
-  // ds_read_b64_tr_b16: lanes 4j .. 4j+3 of a group of 16 address 16 columns of row j; lane l receives column l of the four.
-  static __device__ __forceinline__ Frag colfrag(const bf16* x, int ld, int lane) {
-    const bf16* p = x + (4 * (lane >> 5) + ((lane & 15) >> 2)) * ld + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    typedef __attribute__((address_space(3))) s4v* lp;
-    const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)p);
-    const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 8 * ld));
-    return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-  }
 };
 
 template <>
@@ -75,20 +67,7 @@ struct Mt<float> {  // v_mfma_f32_16x16x4_f32, four of them per fragment
   }
   static __device__ __forceinline__ int crow(int r, int h) { return 4 * h + r; }
   static __device__ __forceinline__ Frag pack(const Acc& s, int) { return s; }
-  static __device__ __forceinline__ Frag colfrag(const float* x, int ld, int lane) {
-    const float* p = x + 4 * (lane >> 4) * ld + (lane & 15);
-    Frag f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = p[i * ld];
-    return f;
-  }
 };
-
-template <typename T>
-__device__ __forceinline__ typename Mt<T>::Frag rowfrag(const T* x, int ld, int lane) {
-  using M = Mt<T>;
-  return *(const typename M::Frag*)(x + (lane & (M::TM - 1)) * ld + M::EP * (lane / M::TM));
-}
 
 // Combination over the lane groups that share a column (lanes n, n + TM, ..).  The values come from vector instructions, not
 // from MFMA results in flight; s_nop 1 covers the distance v_permlane*_swap wants from them.
@@ -124,15 +103,118 @@ __device__ __forceinline__ float col_sum(float v) {
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
 
-// Row strides of the LDS tiles (elements).  Rows read along d: 16 bytes more than a multiple of 64 banks spreads 16 rows over
-// all of them.  bf16 columns (transposed reads touch 4 rows x 64 bytes at a time): 16 banks between rows.
+// ------------------------------------------------------------------------------------------------------ tiles in LDS
+// A tile is rows of CPS 16-byte chunks without padding (the loads below write 1 KB runs), in an order that both ways of
+// reading it find without bank conflicts: row r lies at phys(r), its chunk c in slot c ^ swz(phys(r)).  Sixteen rows read at one
+// chunk (rowfrag) and four rows read at four neighbouring chunks (colfrag) both touch 64 different banks.  phys is the
+// identity for bf16, whose column reads take four neighbouring rows; fp32 takes the rows 4h + i of the four lane groups h at
+// once, so there the two low bit pairs of the row are exchanged.
+constexpr int pow2_up(int x) { return x <= 2 ? 2 : x <= 4 ? 4 : x <= 8 ? 8 : x <= 16 ? 16 : 32; }
+
 template <typename T, int DP>
-struct Ld {
-  static constexpr int DV = (sizeof(T) == 2 && DP < 32) ? 32 : DP;  // columns that whole tiles of the output product cover
-  static constexpr int row = DP + 16 / sizeof(T);
-  static constexpr int col = sizeof(T) == 4 ? DP + 4 : (DV % 128 == 0 ? DV + 32 : DV % 64 == 0 ? DV + 32 : DV);
-  static constexpr int both = DV + 16 / sizeof(T);
+struct Lay {
+  using M = Mt<T>;
+  static constexpr int CPS = pow2_up(DP / M::EP), ROWB = CPS * 16, HG = 64 / M::TM;
+  static constexpr int DV = sizeof(T) == 2 && DP < 32 ? 32 : DP, MD = DV / M::TM, KF = DP / 16;
+  static __device__ __forceinline__ int phys(int r) { return sizeof(T) == 2 ? r : (r & ~15) | (r & 3) << 2 | (r >> 2 & 3); }
+  static __device__ __forceinline__ int swz(int p) {
+    return ROWB == 32 ? p >> 3 & 1 : ROWB == 64 ? p >> 2 & 3 : ROWB == 128 ? (p >> 1 & 1) << 2 | (p >> 2 & 3) : (p & 3) << 2 | (p >> 2 & 3);
+  }
+  // 16 steps of k along d: fragment f of the row that the lane's column index names (rows n .. of a tile at x)
+  static __device__ __forceinline__ typename M::Frag rowfrag(const char* x, int f, int lane) {
+    const int p = phys(lane & (M::TM - 1)), c = HG * f + lane / M::TM;
+    return *(const typename M::Frag*)(x + p * ROWB + (c ^ swz(p)) * 16);
+  }
+  // column tile md of the 16 rows at x, in the order of an accumulator's rows
+  static __device__ __forceinline__ typename M::Frag colfrag(const char* x, int md, int lane) {
+    if constexpr (sizeof(T) == 2) {
+      // ds_read_b64_tr_b16: lanes 4j .. 4j+3 of a group of 16 address 16 columns of row j; lane l receives column l of the
+      // four.  (Of a 16-wide head only half the tile's columns exist; the other lanes read the first half again, unused.)
+      const int r = 4 * (lane >> 5) + (lane >> 2 & 3), c = (4 * md + 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) & (CPS - 1);
+      typedef __attribute__((address_space(3))) s4v* lp;
+      const char* q = x + 8 * (lane & 1);
+      const s4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + r * ROWB + (c ^ swz(r)) * 16));
+      const s4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + (r + 8) * ROWB + (c ^ swz(r + 8)) * 16));
+      return __builtin_bit_cast(typename M::Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      const int h = lane >> 4, c = 4 * md + (lane >> 2 & 3);
+      typename M::Frag f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = *(const float*)(x + (4 * i + h) * ROWB + (c ^ swz(4 * i + h)) * 16 + 4 * (lane & 3));
+      return f;
+    }
+  }
 };
+
+__device__ __attribute__((aligned(16))) unsigned attn_zero[4];  // what hidden rows are read from
+__device__ float attn_inf = INFINITY;
+
+// Asynchronous loads into LDS: lane i's 16 (4) bytes land at lds + 16 i (4 i).  They count as vector memory loads, complete in
+// order, and are waited for by the s_waitcnt of stage_done().
+__device__ __forceinline__ void dma16(const void* p, unsigned lds) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "v"(p), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void dma16(const void* base, unsigned off, unsigned lds) {  // wave-uniform base
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "v"(off), "s"(base), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void dma4(const void* p, unsigned lds) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "v"(p), "s"(lds) : "memory");
+}
+// The wave's own loads but the newest N have landed and its LDS reads are done; BAR: so have the other waves' of the workgroup.
+template <int N, bool BAR>
+__device__ __forceinline__ void stage_done() {
+  if (BAR) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+  else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return (unsigned)(size_t)(__attribute__((address_space(3))) const char*)p;
+}
+
+// ROWS rows of a tile, loaded by NW waves: which of its rows and chunks this lane brings.  A round is one load of every wave
+// (STEP rows); row order and swizzle repeat every 16 rows, so NV rounds cover all different offsets.
+template <typename T, int DP, int ROWS, int NW>
+struct Dma {
+  using L = Lay<T, DP>;
+  static constexpr int RPI = 64 / L::CPS, STEP = RPI * NW, NI = ROWS <= STEP ? 1 : ROWS / STEP, NV = STEP >= 16 ? 1 : 16 / STEP;
+  static_assert(ROWS % RPI == 0 && (ROWS <= STEP || ROWS % STEP == 0) && (NI == 1 || NI % NV == 0), "whole rounds");
+  static constexpr int COUNT = NI;  // loads per wave and tile (none for a wave beyond ROWS)
+  static __device__ __forceinline__ int place(int w, int lane, int i) { return (i * NW + w) * RPI + lane / L::CPS; }
+  static __device__ __forceinline__ int row(int w, int lane, int i) { return L::phys(place(w, lane, i)); }  // phys is its own inverse
+  static __device__ __forceinline__ int chunk(int w, int lane, int i) { return (lane & (L::CPS - 1)) ^ L::swz(place(w, lane, i)); }
+  // all rows are there: uniform base + the lane's offset
+  static __device__ __forceinline__ void whole(const T* base, long long stride, int D, unsigned lds, int w, int lane) {
+    if (ROWS < STEP && w * RPI >= ROWS) return;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int v = i % NV, c = chunk(w, lane, v);
+      const unsigned off = (unsigned)(row(w, lane, v) * (int)stride * (int)sizeof(T) + c * 16);
+      if (c * Mt<T>::EP < D) dma16(base + (long long)(i / NV * NV * STEP) * stride, off, lds + (i * NW + w) * 1024);
+    }
+  }
+  // rows by address: at(r) is the row, or null for one that reads as zero
+  template <typename At>
+  static __device__ __forceinline__ void rows(At at, int D, unsigned lds, int w, int lane) {
+    if (ROWS < STEP && w * RPI >= ROWS) return;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = chunk(w, lane, i);
+      const T* p = at(row(w, lane, i));
+      if (c * Mt<T>::EP < D) dma16(p ? (const void*)(p + c * Mt<T>::EP) : (const void*)attn_zero, lds + (i * NW + w) * 1024);
+    }
+  }
+};
+
+// Chunks at and beyond D are never loaded; a product's zero times whatever stands there has to be zero.
+__device__ __forceinline__ void clear_lds(char* lds, int bytes, int nth) {
+  for (int i = threadIdx.x * 16; i < bytes; i += nth * 16) *(u4v*)(lds + i) = u4v{0, 0, 0, 0};
+  __syncthreads();
+}
 
 struct Strides {
   long long b, l, h;
@@ -142,7 +224,7 @@ struct AttnP {
   const void *q, *k, *v, *dout;
   void *out, *dq, *dk, *dv;
   Strides sq, sk, sv, sdo;
-  float *lse, *delta, *part_o, *part_l;
+  float *lse, *lse2, *delta, *part_o, *part_l;
   const int *lengths, *q_start;
   const unsigned char* key_mask;
   long long mask_sb;
@@ -183,33 +265,6 @@ __device__ __forceinline__ Prob problem(const AttnP& a, int p) {
   return r;
 }
 
-// ROWS rows of DP elements, staged through registers: load() requests them, store() writes them to LDS.  Rows that `ok`
-// refuses are zero and never read: hidden keys may hold anything.
-template <typename T, int DP, int ROWS, int NTH>
-struct Stage {
-  static constexpr int EP = Mt<T>::EP, CPR = DP / EP, N = ROWS * CPR, NCH = (N + NTH - 1) / NTH;
-  u4v r[NCH];
-  template <typename RowPtr>
-  __device__ __forceinline__ void load(int D, RowPtr row) {
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      const int c = threadIdx.x + i * NTH, j = c / CPR, e = (c % CPR) * EP;
-      r[i] = u4v{0, 0, 0, 0};
-      if ((N % NTH == 0 || c < N) && e < D) {
-        const T* p = row(j);
-        if (p) r[i] = *(const u4v*)(p + e);
-      }
-    }
-  }
-  __device__ __forceinline__ void store(T* lds, int ld) const {
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-      const int c = threadIdx.x + i * NTH;
-      if (N % NTH == 0 || c < N) *(u4v*)(lds + (c / CPR) * ld + (c % CPR) * EP) = r[i];
-    }
-  }
-};
-
 // fragments of the stationary rows, straight from global memory (zero where p is null or d >= D)
 template <typename T, int KF>
 __device__ __forceinline__ void load_frags(typename Mt<T>::Frag (&f)[KF], const T* p, int D, int h) {
@@ -241,207 +296,287 @@ __device__ __forceinline__ void store_cols(const typename Mt<T>::Acc (&o)[MD], f
     }
 }
 
-// ---------------------------------------------------------------------------------------------------- forward
-// WM waves along the rows x WK waves along the keys; a wave walks KT keys of every stage of WK * KT.
-template <typename T, int DP, int WM, int WK, int KT, int NBUF>
-struct Fwd {
-  using M = Mt<T>;
-  static constexpr int TM = M::TM, MT = KT / TM, BN = WK * KT, BM = WM * TM, NTH = 64 * WM * WK, KF = DP / 16;
-  static constexpr int DV = Ld<T, DP>::DV, MD = DV / TM, LK = Ld<T, DP>::row, LV = Ld<T, DP>::col, LO = DV + 4;
-  static constexpr size_t stage_bytes = (size_t)NBUF * BN * (LK + LV) * sizeof(T);
-  static constexpr size_t join_bytes = WK > 1 ? (size_t)WK * BM * (LO + 2) * 4 : 0;
-  static constexpr size_t lds = stage_bytes > join_bytes ? stage_bytes : join_bytes;
+// Which keys of a stage (KT <= 64 from j0 on) are there: bit x = key j0 + x.  With a mask its bytes are read a stage ahead.
+template <int KT>
+struct Keys {
+  static constexpr unsigned long long ALL = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
+  const unsigned char* km;
+  int kend;
+  unsigned char byte;
+  __device__ __forceinline__ void fetch(int j0, int lane) {
+    if (km) byte = lane < KT && j0 + lane < kend ? km[j0 + lane] : 0;
+  }
+  __device__ __forceinline__ unsigned long long bits(int j0) const {
+    if (km) return __ballot(byte != 0);
+    const int n = kend - j0;
+    return n >= KT ? ALL : n <= 0 ? 0ull : (1ull << n) - 1;
+  }
 };
 
-extern __shared__ __attribute__((aligned(16))) unsigned char attn_smem[];
+// The tile's rows of keys or values -> LDS; hidden rows are zero and never read (they may hold anything).
+template <typename T, int DP, int KT, int NW>
+__device__ __forceinline__ void load_keys(const T* base, long long stride, int D, int j0, unsigned long long bits, unsigned lds, int w,
+                                          int lane) {
+  using Dm = Dma<T, DP, KT, NW>;
+  const T* b = base + (long long)j0 * stride;
+  if (bits == Keys<KT>::ALL && stride < (1 << 22)) Dm::whole(b, stride, D, lds, w, lane);
+  else Dm::rows([&](int r) { return bits >> r & 1 ? b + (long long)r * stride : (const T*)nullptr; }, D, lds, w, lane);
+}
 
-template <typename T, int DP, int WM, int WK, int KT, int NBUF>
-__global__ void __launch_bounds__(64 * WM * WK, 2) k_attn_fwd(const AttnP a) {
-  using F = Fwd<T, DP, WM, WK, KT, NBUF>;
+// bits of a stage -> the lane's: bit x = its row sees key j0 + x; shifted so that an accumulator's rows are at constant places
+template <int KT>
+__device__ __forceinline__ unsigned long long lane_bits(unsigned long long bits, int j0, int lim, int h) {
+  if (lim < j0 + KT - 1) bits &= lim < j0 ? 0ull : ~0ull >> (63 - (lim - j0));
+  return bits >> (4 * h);
+}
+
+// One stage of the forward: KT keys at ks / vs against the wave's rows.
+template <typename T, int DP, int KT>
+__device__ __forceinline__ void attend(const char* ks, const char* vs, const typename Mt<T>::Frag (&qf)[DP / 16],
+                                       typename Mt<T>::Acc (&o)[Lay<T, DP>::MD], float& m, float& l, unsigned long long bits, int j0,
+                                       int lim, float c, int lane) {
   using M = Mt<T>;
-  constexpr int TM = F::TM, MT = F::MT, BN = F::BN, BM = F::BM, NTH = F::NTH, KF = F::KF, MD = F::MD, LK = F::LK, LV = F::LV;
+  using L = Lay<T, DP>;
+  constexpr int TM = M::TM, MT = KT / TM;
+  typename M::Acc sc[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    sc[mt] = (typename M::Acc)(0.f);
+#pragma unroll
+    for (int f = 0; f < L::KF; ++f) sc[mt] = M::mma(L::rowfrag(ks + mt * TM * L::ROWB, f, lane), qf[f], sc[mt]);
+  }
+  if (bits != Keys<KT>::ALL || __any(lim < j0 + KT - 1)) {
+    bits = lane_bits<KT>(bits, j0, lim, lane / TM);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int r = 0; r < M::NC; ++r)
+        if (!(bits >> (mt * TM + M::crow(r, 0)) & 1)) sc[mt][r] = -INFINITY;
+  }
+  float mx = sc[0][0];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int r = 0; r < M::NC; ++r) mx = fmaxf(mx, sc[mt][r]);
+  // The row's reference moves only when a score exceeds it by 8 powers of two: until then the sums just grow, in fp32, and
+  // the products' operands keep their relative precision.  alpha is 1 for the rows of the wave that stay.
+  mx = col_max<T>(mx);
+  const bool grow = (mx - m) * c > 8.f;  // of a row without a key so far: inf > 8; still without: nan > 8
+  if (__any(grow)) {
+    const float alpha = grow ? exp2_((m - mx) * c) : 1.f;
+    m = grow ? mx : m;
+    l *= alpha;
+#pragma unroll
+    for (int md = 0; md < L::MD; ++md) o[md] *= alpha;
+  }
+  const float mc = m == -INFINITY ? 0.f : m * c;
+  float sum = 0.f;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int r = 0; r < M::NC; ++r) {
+      const float e = exp2_(__builtin_fmaf(sc[mt][r], c, -mc));
+      sc[mt][r] = e;
+      sum += e;
+    }
+  l += sum;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int t = 0; t < TM / 16; ++t) {
+      const typename M::Frag pf = M::pack(sc[mt], t);
+#pragma unroll
+      for (int md = 0; md < L::MD; ++md)
+        o[md] = M::mma(L::colfrag(vs + (mt * TM + 16 * t) * L::ROWB, md, lane), pf, o[md]);
+    }
+}
+
+extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
+
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+// what a forward workgroup needs to know of its rows
+struct Rows {
+  int row, i, g, hq, lim, kbeg, kend;
+  bool live;
+};
+__device__ __forceinline__ Rows rows_of(const AttnP& a, const Prob& p, int row0, int row, int nrows, int split) {
+  Rows r;
+  r.row = row, r.live = row < a.M;
+  r.i = row_pos(a, r.live ? row : 0), r.g = (r.live ? row : 0) - r.i * a.G, r.hq = p.hk * a.G + r.g;
+  r.lim = a.causal ? p.qs + r.i : INT_MAX;  // last key the row may see
+  r.kbeg = 0, r.kend = p.len;
+  if (a.causal) r.kend = min(r.kend, p.qs + row_pos(a, min(row0 + nrows, a.M) - 1) + 1);
+  if (a.nsplit > 1) r.kbeg = split * a.split_keys, r.kend = min(r.kend, r.kbeg + a.split_keys);
+  return r;
+}
+
+// ---------------------------------------------------------------------------------------------------- forward
+// NW waves with TM rows each share stages of KT keys and values: while one stage is worked on, the next lands in LDS.
+template <typename T, int DP, int NW, int KT>
+struct Fwd {
+  using L = Lay<T, DP>;
+  static constexpr int TM = Mt<T>::TM, BM = NW * TM, NTH = 64 * NW, TILE = KT * L::ROWB;
+  static constexpr size_t lds = 4 * TILE;  // two stages of keys and values
+};
+
+template <typename T, int DP, int NW, int KT>
+__global__ void __launch_bounds__(64 * NW, 2) k_attn_fwd(const AttnP a) {
+  using F = Fwd<T, DP, NW, KT>;
+  using M = Mt<T>;
+  using L = Lay<T, DP>;
   int pr, unit;
   if (!locate(a.B * a.Hkv, a.tiles * a.nsplit, pr, unit)) return;
   const int split = unit / a.tiles, tile = a.tiles - 1 - (unit - split * a.tiles);  // causal: the longest tiles first
   const Prob p = problem(a, pr);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wk = wave % WK, wm = wave / WK;
-  const int n = lane & (TM - 1), h = lane / TM;
-  const int row = tile * BM + wm * TM + n;
-  const bool live = row < a.M;
-  const int i = row_pos(a, live ? row : 0), g = (live ? row : 0) - i * a.G, hq = p.hk * a.G + g;
-  const int lim = a.causal ? p.qs + i : INT_MAX;  // last key this row may see
-
-  int kend = p.len;
-  if (a.causal) kend = min(kend, p.qs + row_pos(a, min(tile * BM + BM, a.M) - 1) + 1);
-  int kbeg = 0;
-  if (a.nsplit > 1) kbeg = split * a.split_keys, kend = min(kend, kbeg + a.split_keys);
-
-  typename M::Frag qf[KF];
-  load_frags<T, KF>(qf, live ? (const T*)a.q + p.b * a.sq.b + i * a.sq.l + hq * a.sq.h : nullptr, a.D, h);
+  const int lane = threadIdx.x & 63, wave = wave_index(), n = lane & (M::TM - 1), h = lane / M::TM;
+  const Rows r = rows_of(a, p, tile * F::BM, tile * F::BM + wave * M::TM + n, F::BM, split);
+  if (a.D * (int)sizeof(T) < L::ROWB) clear_lds(attn_smem, (int)F::lds, F::NTH);
 
   const T* kb = (const T*)a.k + p.b * a.sk.b + p.hk * a.sk.h;
   const T* vb = (const T*)a.v + p.b * a.sv.b + p.hk * a.sv.h;
-  const unsigned char* km = a.key_mask ? a.key_mask + p.b * a.mask_sb : nullptr;
-  T* ks = (T*)attn_smem;
-  T* vs = ks + NBUF * BN * LK;
-  Stage<T, DP, BN, NTH> sk, sv;
-  const auto request = [&](int j0) {
-    sk.load(a.D, [&](int j) { return j0 + j < kend && (!km || km[j0 + j]) ? kb + (j0 + j) * a.sk.l : (const T*)nullptr; });
-    sv.load(a.D, [&](int j) { return j0 + j < kend && (!km || km[j0 + j]) ? vb + (j0 + j) * a.sv.l : (const T*)nullptr; });
+  const unsigned base = lds_address(attn_smem);
+  Keys<KT> keys = {a.key_mask ? a.key_mask + p.b * a.mask_sb : nullptr, r.kend, 0};
+  const auto request = [&](int j0, unsigned long long bits, int buf) {
+    load_keys<T, DP, KT, NW>(kb, a.sk.l, a.D, j0, bits, base + buf * 2 * F::TILE, wave, lane);
+    load_keys<T, DP, KT, NW>(vb, a.sv.l, a.D, j0, bits, base + (buf * 2 + 1) * F::TILE, wave, lane);
   };
-  const int stages = kend > kbeg ? (kend - kbeg + BN - 1) / BN : 0;
+  keys.fetch(r.kbeg, lane);
+  unsigned long long bits = keys.bits(r.kbeg), next = 0;
+  if (bits) request(r.kbeg, bits, 0);
+  keys.fetch(r.kbeg + KT, lane);
 
-  typename M::Acc o[MD];
+  typename M::Frag qf[L::KF];
+  load_frags<T, L::KF>(qf, r.live ? (const T*)a.q + p.b * a.sq.b + r.i * a.sq.l + r.hq * a.sq.h : nullptr, a.D, h);
+  typename M::Acc o[L::MD];
 #pragma unroll
-  for (int md = 0; md < MD; ++md) o[md] = (typename M::Acc)(0.f);
-  float m = -INFINITY, l = 0.f;  // running maximum of the raw scores; this lane's share of the sum
-
-  if (stages) {
-    request(kbeg);
-    if (NBUF == 2) {
-      sk.store(ks, LK), sv.store(vs, LV);
-      if (stages > 1) request(kbeg + BN);
-      __syncthreads();
-    }
-  }
-  for (int s = 0; s < stages; ++s) {
-    const int j0 = kbeg + s * BN;
-    if (NBUF == 2) {
-      if (s + 1 < stages) {
-        sk.store(ks + ((s + 1) & 1) * BN * LK, LK), sv.store(vs + ((s + 1) & 1) * BN * LV, LV);
-        if (s + 2 < stages) request(j0 + 2 * BN);
-      }
-    } else {
-      sk.store(ks, LK), sv.store(vs, LV);
-      __syncthreads();
-      if (s + 1 < stages) request(j0 + BN);
-    }
-    const T* kt = ks + (NBUF == 2 ? (s & 1) * BN * LK : 0) + wk * KT * LK;
-    const T* vt = vs + (NBUF == 2 ? (s & 1) * BN * LV : 0) + wk * KT * LV;
-    const int jw = j0 + wk * KT;
-    const bool key_ok = lane < KT && jw + lane < kend && (!km || km[jw + lane]);
-    unsigned long long bits = __ballot(key_ok);
-    if (bits && !__all(lim < jw)) {
-      typename M::Acc sc[MT];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        sc[mt] = (typename M::Acc)(0.f);
-#pragma unroll
-        for (int f = 0; f < KF; ++f) sc[mt] = M::mma(rowfrag<T>(kt + mt * TM * LK + 16 * f, LK, lane), qf[f], sc[mt]);
-      }
-      constexpr unsigned long long ALL = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
-      if (bits != ALL || __any(lim < jw + KT - 1)) {
-        // bit x of the lane: key jw + x is visible to its row
-        if (lim < jw + KT - 1) bits &= lim < jw ? 0ull : ~0ull >> (63 - (lim - jw));
-        bits >>= 4 * h;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int r = 0; r < M::NC; ++r)
-            if (!(bits >> (mt * TM + M::crow(r, 0)) & 1)) sc[mt][r] = -INFINITY;
-      }
-      float mx = sc[0][0];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int r = 0; r < M::NC; ++r) mx = fmaxf(mx, sc[mt][r]);
-      // The row's reference moves only when a score exceeds it by 8 powers of two: until then the sums just grow, in fp32, and
-      // the products' operands keep their relative precision.  alpha is 1 for the rows of the wave that stay.
-      mx = col_max<T>(mx);
-      const bool grow = (mx - m) * a.c > 8.f;  // of a row without a key so far: inf > 8; still without: nan > 8
-      if (__any(grow)) {
-        const float alpha = grow ? exp2_((m - mx) * a.c) : 1.f;
-        m = grow ? mx : m;
-        l *= alpha;
-#pragma unroll
-        for (int md = 0; md < MD; ++md) o[md] *= alpha;
-      }
-      const float mc = m == -INFINITY ? 0.f : m * a.c;
-      float sum = 0.f;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int r = 0; r < M::NC; ++r) {
-          const float e = exp2_(__builtin_fmaf(sc[mt][r], a.c, -mc));
-          sc[mt][r] = e;
-          sum += e;
-        }
-      l += sum;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int t = 0; t < TM / 16; ++t) {
-          const typename M::Frag pf = M::pack(sc[mt], t);
-#pragma unroll
-          for (int md = 0; md < MD; ++md)
-            o[md] = M::mma(M::colfrag(vt + (mt * TM + 16 * t) * LV + md * TM, LV, lane), pf, o[md]);
-        }
-    }
-    __syncthreads();
+  for (int md = 0; md < L::MD; ++md) o[md] = (typename M::Acc)(0.f);
+  float m = -INFINITY, l = 0.f;  // reference of the raw scores; this lane's share of the sum
+  stage_done<0, true>();
+  int buf = 0;
+  for (int j0 = r.kbeg; j0 < r.kend; j0 += KT, buf ^= 1, bits = next) {
+    next = keys.bits(j0 + KT);
+    keys.fetch(j0 + 2 * KT, lane);
+    if (next) request(j0 + KT, next, buf ^ 1);
+    if (bits && !__all(r.lim < j0))
+      attend<T, DP, KT>(attn_smem + buf * 2 * F::TILE, attn_smem + (buf * 2 + 1) * F::TILE, qf, o, m, l, bits, j0, r.lim, a.c, lane);
+    stage_done<0, true>();
   }
   l = col_sum<T>(l);
-
-  if (WK > 1) {  // join the waves that walked different keys
-    constexpr int LO = F::LO;
-    float* mo = (float*)attn_smem;  // [WK][BM] maxima, [WK][BM] sums, [WK][BM][LO] outputs
-    float* lo = mo + WK * BM;
-    float* oo = lo + WK * BM;
-    // every wave is past its last read of the stages (the barrier that ends the loop; without a stage nothing was read)
-    if (h == 0) mo[wk * BM + wm * TM + n] = m, lo[wk * BM + wm * TM + n] = l;
-#pragma unroll
-    for (int md = 0; md < MD; ++md)
-#pragma unroll
-      for (int q = 0; q < M::NC / 4; ++q) {
-        fl4 x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = o[md][4 * q + e];
-        *(fl4*)(oo + (wk * BM + wm * TM + n) * LO + md * TM + M::crow(4 * q, h)) = x;
-      }
-    __syncthreads();
-    for (int x = threadIdx.x; x < BM * (DP / 4); x += NTH) {
-      const int rr = x / (DP / 4), d = 4 * (x % (DP / 4)), rw = tile * BM + rr;
-      if (rw >= a.M) continue;
-      float mm = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < WK; ++w) mm = fmaxf(mm, mo[w * BM + rr]);
-      const float ms = mm == -INFINITY ? 0.f : mm;
-      float ll = 0.f;
-      fl4 acc = (fl4)(0.f);
-#pragma unroll
-      for (int w = 0; w < WK; ++w) {
-        const float f = exp2_((mo[w * BM + rr] - ms) * a.c);
-        ll += f * lo[w * BM + rr];
-        acc += f * *(const fl4*)(oo + (w * BM + rr) * LO + d);
-      }
-      acc *= ll > 0.f || ll != ll ? 1.f / ll : 0.f;
-      const float l2 = ll == 0.f ? -INFINITY : ms * a.c + log2_(ll);
-      const int ii = row_pos(a, rw), hh = p.hk * a.G + rw - ii * a.G;
-      if (a.nsplit > 1) {
-        const long long at = ((long long)split * a.B * a.Hkv + pr) * a.M + rw;
-        if (d == 0) a.part_l[at] = l2;
-        if (d < a.D) *(fl4*)(a.part_o + at * a.D + d) = acc;
-      } else {
-        if (d == 0) a.lse[((long long)p.b * a.Hq + hh) * a.Lq + ii] = l2 * LN2;
-        typedef T V4 __attribute__((ext_vector_type(4)));
-        V4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = (T)acc[e];
-        if (d < a.D) *(V4*)((T*)a.out + (((long long)p.b * a.Lq + ii) * a.Hq + hh) * a.D + d) = y;
-      }
-    }
-    return;
-  }
-  if (!live) return;
+  if (!r.live) return;
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // a row without a key is zero
   const float l2 = l == 0.f ? -INFINITY : m * a.c + log2_(l);
   if (a.nsplit > 1) {
-    const long long at = ((long long)split * a.B * a.Hkv + pr) * a.M + row;
+    const long long at = ((long long)split * a.B * a.Hkv + pr) * a.M + r.row;
     if (h == 0) a.part_l[at] = l2;
-    store_cols<T, float, MD>(o, inv, a.part_o + at * a.D, a.D, h);
+    store_cols<T, float, L::MD>(o, inv, a.part_o + at * a.D, a.D, h);
     return;
   }
-  if (h == 0) a.lse[((long long)p.b * a.Hq + hq) * a.Lq + i] = l2 * LN2;
-  store_cols<T, T, MD>(o, inv, (T*)a.out + (((long long)p.b * a.Lq + i) * a.Hq + hq) * a.D, a.D, h);
+  if (h == 0) a.lse[((long long)p.b * a.Hq + r.hq) * a.Lq + r.i] = l2 * LN2;
+  store_cols<T, T, L::MD>(o, inv, (T*)a.out + (((long long)p.b * a.Lq + r.i) * a.Hq + r.hq) * a.D, a.D, h);
+}
+
+// Few rows (one tile of them, e.g. one new token of a sequence): the WK waves share the rows and divide the keys, each with
+// stages of its own and no barrier until their sums are joined.
+template <typename T, int DP, int WK, int KT>
+struct Few {
+  using L = Lay<T, DP>;
+  static constexpr int TM = Mt<T>::TM, NTH = 64 * WK, TILE = KT * L::ROWB, LO = L::DV + 4;
+  static constexpr size_t stage_bytes = (size_t)WK * 4 * TILE, join_bytes = (size_t)WK * TM * (LO + 2) * 4;
+  static constexpr size_t lds = stage_bytes > join_bytes ? stage_bytes : join_bytes;
+};
+
+template <typename T, int DP, int WK, int KT>
+__global__ void __launch_bounds__(64 * WK, 2) k_attn_few(const AttnP a) {
+  using F = Few<T, DP, WK, KT>;
+  using M = Mt<T>;
+  using L = Lay<T, DP>;
+  constexpr int TM = M::TM, LO = F::LO;
+  int pr, split;
+  if (!locate(a.B * a.Hkv, a.nsplit, pr, split)) return;
+  const Prob p = problem(a, pr);
+  const int lane = threadIdx.x & 63, wave = wave_index(), n = lane & (TM - 1), h = lane / TM;
+  const Rows r = rows_of(a, p, 0, n, TM, split);
+  if (a.D * (int)sizeof(T) < L::ROWB) clear_lds(attn_smem, (int)F::stage_bytes, F::NTH);
+
+  const T* kb = (const T*)a.k + p.b * a.sk.b + p.hk * a.sk.h;
+  const T* vb = (const T*)a.v + p.b * a.sv.b + p.hk * a.sv.h;
+  const char* mine = attn_smem + wave * 4 * F::TILE;
+  const unsigned base = lds_address(attn_smem) + wave * 4 * F::TILE;
+  Keys<KT> keys = {a.key_mask ? a.key_mask + p.b * a.mask_sb : nullptr, r.kend, 0};
+  const auto request = [&](int j0, unsigned long long bits, int buf) {
+    load_keys<T, DP, KT, 1>(kb, a.sk.l, a.D, j0, bits, base + buf * 2 * F::TILE, 0, lane);
+    load_keys<T, DP, KT, 1>(vb, a.sv.l, a.D, j0, bits, base + (buf * 2 + 1) * F::TILE, 0, lane);
+  };
+  const int jb = r.kbeg + wave * KT;
+  keys.fetch(jb, lane);
+  unsigned long long bits = keys.bits(jb), next = 0;
+  if (bits) request(jb, bits, 0);
+  keys.fetch(jb + WK * KT, lane);
+  typename M::Frag qf[L::KF];
+  load_frags<T, L::KF>(qf, r.live ? (const T*)a.q + p.b * a.sq.b + r.i * a.sq.l + r.hq * a.sq.h : nullptr, a.D, h);
+  typename M::Acc o[L::MD];
+#pragma unroll
+  for (int md = 0; md < L::MD; ++md) o[md] = (typename M::Acc)(0.f);
+  float m = -INFINITY, l = 0.f;
+  stage_done<0, false>();
+  int buf = 0;
+  for (int j0 = jb; j0 < r.kend; j0 += WK * KT, buf ^= 1, bits = next) {
+    next = keys.bits(j0 + WK * KT);
+    keys.fetch(j0 + 2 * WK * KT, lane);
+    if (next) request(j0 + WK * KT, next, buf ^ 1);
+    if (bits && !__all(r.lim < j0))
+      attend<T, DP, KT>(mine + buf * 2 * F::TILE, mine + (buf * 2 + 1) * F::TILE, qf, o, m, l, bits, j0, r.lim, a.c, lane);
+    stage_done<0, false>();
+  }
+  l = col_sum<T>(l);
+
+  float* mo = (float*)attn_smem;  // [WK][TM] references, [WK][TM] sums, [WK][TM][LO] outputs
+  float* lo = mo + WK * TM;
+  float* oo = lo + WK * TM;
+  __syncthreads();  // every wave is past its last stage
+  if (h == 0) mo[wave * TM + n] = m, lo[wave * TM + n] = l;
+#pragma unroll
+  for (int md = 0; md < L::MD; ++md)
+#pragma unroll
+    for (int q = 0; q < M::NC / 4; ++q) {
+      fl4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = o[md][4 * q + e];
+      *(fl4*)(oo + (wave * TM + n) * LO + md * TM + M::crow(4 * q, h)) = x;
+    }
+  __syncthreads();
+  for (int x = threadIdx.x; x < TM * (DP / 4); x += F::NTH) {
+    const int rw = x / (DP / 4), d = 4 * (x % (DP / 4));
+    if (rw >= a.M) continue;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) mm = fmaxf(mm, mo[w * TM + rw]);
+    const float ms = mm == -INFINITY ? 0.f : mm;
+    float ll = 0.f;
+    fl4 acc = (fl4)(0.f);
+#pragma unroll
+    for (int w = 0; w < WK; ++w) {
+      const float f = exp2_((mo[w * TM + rw] - ms) * a.c);
+      ll += f * lo[w * TM + rw];
+      acc += f * *(const fl4*)(oo + (w * TM + rw) * LO + d);
+    }
+    acc *= ll > 0.f || ll != ll ? 1.f / ll : 0.f;
+    const float l2 = ll == 0.f ? -INFINITY : ms * a.c + log2_(ll);
+    const int i = row_pos(a, rw), hq = p.hk * a.G + rw - i * a.G;
+    if (a.nsplit > 1) {
+      const long long at = ((long long)split * a.B * a.Hkv + pr) * a.M + rw;
+      if (d == 0) a.part_l[at] = l2;
+      if (d < a.D) *(fl4*)(a.part_o + at * a.D + d) = acc;
+    } else {
+      if (d == 0) a.lse[((long long)p.b * a.Hq + hq) * a.Lq + i] = l2 * LN2;
+      typedef T V4 __attribute__((ext_vector_type(4)));
+      V4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = (T)acc[e];
+      if (d < a.D) *(V4*)((T*)a.out + (((long long)p.b * a.Lq + i) * a.Hq + hq) * a.D + d) = y;
+    }
+  }
 }
 
 // Joins the splits of a row: every split left its own normalised output and log2-sum-exp.  32 lanes per row, 4 values a lane.
@@ -478,111 +613,92 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnP a) {
 // ---------------------------------------------------------------------------------------------------- gradient of queries
 // Rows of queries and of the output's gradient are stationary; keys and values walk past.  The probabilities are computed
 // again from the row's log-sum-exp, so a row's share of the work needs no maximum and no sum:
-//   p = exp(s - lse), ds = p (do.v - delta), dq = scale sum ds k,  delta = do.o  (written out for the other kernel).
-template <typename T, int DP, int WM, int KT>
-struct Dq {
+//   p = exp(s - lse), ds = p (do.v - delta), dq = scale sum ds k,  delta = do.o
+// delta and the log-sum-exp in powers of two (+inf for a row without a key) are left for the other kernel.
+template <typename T, int DP, int NW, int KT>
+__global__ void __launch_bounds__(64 * NW, 2) k_attn_dq(const AttnP a) {
+  using F = Fwd<T, DP, NW, KT>;
   using M = Mt<T>;
-  static constexpr int TM = M::TM, MT = KT / TM, BM = WM * TM, NTH = 64 * WM, KF = DP / 16;
-  static constexpr int DV = Ld<T, DP>::DV, MD = DV / TM, LK = Ld<T, DP>::both, LV = Ld<T, DP>::row;
-  static constexpr size_t lds = (size_t)2 * KT * (LK + LV) * sizeof(T);
-};
-
-template <typename T, int DP, int WM, int KT>
-__global__ void __launch_bounds__(64 * WM, 2) k_attn_dq(const AttnP a) {
-  using F = Dq<T, DP, WM, KT>;
-  using M = Mt<T>;
-  constexpr int TM = F::TM, MT = F::MT, BM = F::BM, NTH = F::NTH, KF = F::KF, MD = F::MD, LK = F::LK, LV = F::LV;
+  using L = Lay<T, DP>;
+  constexpr int TM = M::TM, MT = KT / TM;
   int pr, unit;
   if (!locate(a.B * a.Hkv, a.tiles, pr, unit)) return;
   const int tile = a.tiles - 1 - unit;
   const Prob p = problem(a, pr);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n = lane & (TM - 1), h = lane / TM;
-  const int row = tile * BM + wave * TM + n;
-  const bool live = row < a.M;
-  const int i = row_pos(a, live ? row : 0), g = (live ? row : 0) - i * a.G, hq = p.hk * a.G + g;
-  const int lim = a.causal ? p.qs + i : INT_MAX;
-  int kend = p.len;
-  if (a.causal) kend = min(kend, p.qs + row_pos(a, min(tile * BM + BM, a.M) - 1) + 1);
+  const int lane = threadIdx.x & 63, wave = wave_index(), n = lane & (TM - 1), h = lane / TM;
+  const Rows r = rows_of(a, p, tile * F::BM, tile * F::BM + wave * TM + n, F::BM, 0);
+  if (a.D * (int)sizeof(T) < L::ROWB) clear_lds(attn_smem, (int)F::lds, F::NTH);
 
-  typename M::Frag qf[KF], df[KF];
-  load_frags<T, KF>(qf, live ? (const T*)a.q + p.b * a.sq.b + i * a.sq.l + hq * a.sq.h : nullptr, a.D, h);
-  load_frags<T, KF>(df, live ? (const T*)a.dout + p.b * a.sdo.b + i * a.sdo.l + hq * a.sdo.h : nullptr, a.D, h);
-  const long long at = ((long long)p.b * a.Hq + hq) * a.Lq + i, orow = (((long long)p.b * a.Lq + i) * a.Hq + hq) * a.D;
+  const T* kb = (const T*)a.k + p.b * a.sk.b + p.hk * a.sk.h;
+  const T* vb = (const T*)a.v + p.b * a.sv.b + p.hk * a.sv.h;
+  const unsigned base = lds_address(attn_smem);
+  Keys<KT> keys = {a.key_mask ? a.key_mask + p.b * a.mask_sb : nullptr, r.kend, 0};
+  const auto request = [&](int j0, unsigned long long bits, int buf) {
+    load_keys<T, DP, KT, NW>(kb, a.sk.l, a.D, j0, bits, base + buf * 2 * F::TILE, wave, lane);
+    load_keys<T, DP, KT, NW>(vb, a.sv.l, a.D, j0, bits, base + (buf * 2 + 1) * F::TILE, wave, lane);
+  };
+  keys.fetch(0, lane);
+  unsigned long long bits = keys.bits(0), next = 0;
+  if (bits) request(0, bits, 0);
+  keys.fetch(KT, lane);
+
+  typename M::Frag qf[L::KF], df[L::KF];
+  load_frags<T, L::KF>(qf, r.live ? (const T*)a.q + p.b * a.sq.b + r.i * a.sq.l + r.hq * a.sq.h : nullptr, a.D, h);
+  load_frags<T, L::KF>(df, r.live ? (const T*)a.dout + p.b * a.sdo.b + r.i * a.sdo.l + r.hq * a.sdo.h : nullptr, a.D, h);
+  const long long at = ((long long)p.b * a.Hq + r.hq) * a.Lq + r.i, orow = (((long long)p.b * a.Lq + r.i) * a.Hq + r.hq) * a.D;
   float delta = 0.f;
   {
-    typename M::Frag of[KF];
-    load_frags<T, KF>(of, live ? (const T*)a.out + orow : nullptr, a.D, h);
+    typename M::Frag of[L::KF];
+    load_frags<T, L::KF>(of, r.live ? (const T*)a.out + orow : nullptr, a.D, h);
 #pragma unroll
-    for (int f = 0; f < KF; ++f)
+    for (int f = 0; f < L::KF; ++f)
 #pragma unroll
       for (int e = 0; e < M::EP; ++e) delta = __builtin_fmaf((float)df[f][e], (float)of[f][e], delta);
     delta = col_sum<T>(delta);
   }
-  float lse2 = live ? a.lse[at] * LOG2E : INFINITY;
+  float lse2 = r.live ? a.lse[at] * LOG2E : INFINITY;
   if (lse2 == -INFINITY) lse2 = INFINITY;  // a row without a key: every probability is zero
-  if (live && h == 0) a.delta[at] = delta;
+  if (r.live && h == 0) a.delta[at] = delta, a.lse2[at] = lse2;
 
-  const T* kb = (const T*)a.k + p.b * a.sk.b + p.hk * a.sk.h;
-  const T* vb = (const T*)a.v + p.b * a.sv.b + p.hk * a.sv.h;
-  const unsigned char* km = a.key_mask ? a.key_mask + p.b * a.mask_sb : nullptr;
-  T* ks = (T*)attn_smem;
-  T* vs = ks + 2 * KT * LK;
-  Stage<T, DP, KT, NTH> sk, sv;
-  const auto request = [&](int j0) {
-    sk.load(a.D, [&](int j) { return j0 + j < kend && (!km || km[j0 + j]) ? kb + (j0 + j) * a.sk.l : (const T*)nullptr; });
-    sv.load(a.D, [&](int j) { return j0 + j < kend && (!km || km[j0 + j]) ? vb + (j0 + j) * a.sv.l : (const T*)nullptr; });
-  };
-  const int stages = kend > 0 ? (kend + KT - 1) / KT : 0;
-  typename M::Acc dq[MD];
+  typename M::Acc dq[L::MD];
 #pragma unroll
-  for (int md = 0; md < MD; ++md) dq[md] = (typename M::Acc)(0.f);
-  if (stages) {
-    request(0);
-    sk.store(ks, LK), sv.store(vs, LV);
-    if (stages > 1) request(KT);
-    __syncthreads();
-  }
-  for (int s = 0; s < stages; ++s) {
-    const int j0 = s * KT;
-    if (s + 1 < stages) {
-      sk.store(ks + ((s + 1) & 1) * KT * LK, LK), sv.store(vs + ((s + 1) & 1) * KT * LV, LV);
-      if (s + 2 < stages) request(j0 + 2 * KT);
-    }
-    const T* kt = ks + (s & 1) * KT * LK;
-    const T* vt = vs + (s & 1) * KT * LV;
-    unsigned long long bits = __ballot(lane < KT && j0 + lane < kend && (!km || km[j0 + lane]));
-    if (bits && !__all(lim < j0)) {
-      constexpr unsigned long long ALL = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
-      const bool partly = bits != ALL || __any(lim < j0 + KT - 1);
-      if (lim < j0 + KT - 1) bits &= lim < j0 ? 0ull : ~0ull >> (63 - (lim - j0));
-      bits >>= 4 * h;
+  for (int md = 0; md < L::MD; ++md) dq[md] = (typename M::Acc)(0.f);
+  stage_done<0, true>();
+  int buf = 0;
+  for (int j0 = 0; j0 < r.kend; j0 += KT, buf ^= 1, bits = next) {
+    next = keys.bits(j0 + KT);
+    keys.fetch(j0 + 2 * KT, lane);
+    if (next) request(j0 + KT, next, buf ^ 1);
+    if (bits && !__all(r.lim < j0)) {
+      const bool partly = bits != Keys<KT>::ALL || __any(r.lim < j0 + KT - 1);
+      const unsigned long long lb = lane_bits<KT>(bits, j0, r.lim, h);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
+        const char* kt = attn_smem + buf * 2 * F::TILE + mt * TM * L::ROWB;
+        const char* vt = kt + F::TILE;
         typename M::Acc sc = (typename M::Acc)(0.f), dp = (typename M::Acc)(0.f);
 #pragma unroll
-        for (int f = 0; f < KF; ++f) {
-          sc = M::mma(rowfrag<T>(kt + mt * TM * LK + 16 * f, LK, lane), qf[f], sc);
-          dp = M::mma(rowfrag<T>(vt + mt * TM * LV + 16 * f, LV, lane), df[f], dp);
+        for (int f = 0; f < L::KF; ++f) {
+          sc = M::mma(L::rowfrag(kt, f, lane), qf[f], sc);
+          dp = M::mma(L::rowfrag(vt, f, lane), df[f], dp);
         }
 #pragma unroll
-        for (int r = 0; r < M::NC; ++r) {
-          float e = exp2_(__builtin_fmaf(sc[r], a.c, -lse2));
-          if (partly && !(bits >> (mt * TM + M::crow(r, 0)) & 1)) e = 0.f;
-          sc[r] = e * (dp[r] - delta);
+        for (int x = 0; x < M::NC; ++x) {
+          float e = exp2_(__builtin_fmaf(sc[x], a.c, -lse2));
+          if (partly && !(lb >> (mt * TM + M::crow(x, 0)) & 1)) e = 0.f;
+          sc[x] = e * (dp[x] - delta);
         }
 #pragma unroll
         for (int t = 0; t < TM / 16; ++t) {
           const typename M::Frag sf = M::pack(sc, t);
 #pragma unroll
-          for (int md = 0; md < MD; ++md)
-            dq[md] = M::mma(M::colfrag(kt + (mt * TM + 16 * t) * LK + md * TM, LK, lane), sf, dq[md]);
+          for (int md = 0; md < L::MD; ++md) dq[md] = M::mma(L::colfrag(kt + 16 * t * L::ROWB, md, lane), sf, dq[md]);
         }
       }
     }
-    __syncthreads();
+    stage_done<0, true>();
   }
-  if (live) store_cols<T, T, MD>(dq, a.scale, (T*)a.dq + orow, a.D, h);
+  if (r.live) store_cols<T, T, L::MD>(dq, a.scale, (T*)a.dq + orow, a.D, h);
 }
 
 // ---------------------------------------------------------------------------------------------- gradients of keys, values
@@ -595,122 +711,120 @@ __global__ void __launch_bounds__(64 * WM, 2) k_attn_dq(const AttnP a) {
 template <typename T, int DP, int WN, int WR>
 struct Dkv {
   using M = Mt<T>;
-  static constexpr int TM = M::TM, RW = sizeof(T) == 4 && DP > 64 ? 16 : 32, RB = WR * RW, MT = RW / TM, BN = WN * TM, NTH = 64 * WN * WR, KF = DP / 16;
-  static constexpr int DV = Ld<T, DP>::DV, MD = DV / TM, LQ = Ld<T, DP>::both, LV = Ld<T, DP>::row;
+  using L = Lay<T, DP>;
+  static constexpr int TM = M::TM, RW = sizeof(T) == 4 && DP > 64 ? 16 : 32, RB = WR * RW, MT = RW / TM, BN = WN * TM;
+  static constexpr int NW = WN * WR, NTH = 64 * NW, TILE = RB * L::ROWB, STAGE = 2 * TILE, NBUF = 3;
   static constexpr bool VL = DP > 64;
-  static constexpr size_t stage_bytes = (size_t)2 * (2 * RB * LQ * sizeof(T) + 2 * RB * 4) + (VL ? BN * LV * sizeof(T) : 0);
-  static constexpr size_t join_bytes = WR > 1 ? (size_t)WN * 2 * MD * M::NC * 64 * 4 : 0;
+  static constexpr int stats_at = NBUF * STAGE, v_at = stats_at + NBUF * 512;  // [NBUF][2][64] floats; values
+  static constexpr size_t stage_bytes = v_at + (VL ? BN * L::ROWB : 0);
+  static constexpr size_t join_bytes = WR > 1 ? (size_t)WN * 2 * L::MD * M::NC * 64 * 4 : 0;
   static constexpr size_t lds = stage_bytes > join_bytes ? stage_bytes : join_bytes;
+  static constexpr int LOADS = 2 * Dma<T, DP, RB, NW>::COUNT;  // of a wave per stage: this many, one more, or (no rows for it) none
 };
 
 template <typename T, int DP, int WN, int WR>
 __global__ void __launch_bounds__(64 * WN * WR, 2) k_attn_dkv(const AttnP a) {
   using F = Dkv<T, DP, WN, WR>;
   using M = Mt<T>;
+  using L = Lay<T, DP>;
   static_assert(WR == 1 || WR == 2, "the join below exchanges between two waves");
-  constexpr int TM = F::TM, MT = F::MT, RB = F::RB, BN = F::BN, NTH = F::NTH, KF = F::KF, MD = F::MD, LQ = F::LQ, LV = F::LV;
+  static_assert(F::RB <= 64, "one wave brings a stage's row statistics");
+  constexpr int TM = F::TM, MT = F::MT, RB = F::RB, BN = F::BN, KF = L::KF, MD = L::MD, NW = F::NW;
   constexpr bool VL = F::VL;
+  using Dm = Dma<T, DP, RB, NW>;
   int pr, unit;
   if (!locate(a.B * a.Hkv, (a.causal ? (a.tiles + 1) / 2 : a.tiles) * a.nsplit, pr, unit)) return;
   const int tu = unit / a.nsplit, split = unit - tu * a.nsplit;
   const Prob p = problem(a, pr);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave % WN, wr = wave / WN;
+  const int lane = threadIdx.x & 63, wave = wave_index(), wn = wave % WN, wr = wave / WN;
   const int n = lane & (TM - 1), h = lane / TM;
   const unsigned char* km = a.key_mask ? a.key_mask + p.b * a.mask_sb : nullptr;
   const auto first_row = [&](int j) { return !a.causal || j <= p.qs ? 0 : j - p.qs >= a.Lq ? INT_MAX : (j - p.qs) * a.G; };
+  const unsigned base = lds_address(attn_smem);
+  const float* stats = (const float*)(attn_smem + F::stats_at);
+  const char* vw = attn_smem + F::v_at + wn * TM * L::ROWB;
 
-  T* qs = (T*)attn_smem;                   // [2][RB][LQ]
-  T* ds = qs + 2 * RB * LQ;                // [2][RB][LQ]
-  float* ls = (float*)(ds + 2 * RB * LQ);  // [2][RB] log-sum-exp (log2), [2][RB] delta
-  T* vs = (T*)(ls + 4 * RB);               // [BN][LV]
-  Stage<T, DP, RB, NTH> sq, sd;
-  float rl, rd;
-  const auto request = [&](int r0) {
-    const auto at = [&](const void* base, const Strides& s, int r) -> const T* {
-      r += r0;
-      if (r >= a.M) return nullptr;
+  // Rows at and behind M are those of row M - 1 again, with a probability of zero.
+  const auto request = [&](int r0, int buf) {
+    const auto at = [&](const void* x, const Strides& s, int r) {
+      r = min(r0 + r, a.M - 1);
       const int i = row_pos(a, r);
-      return (const T*)base + p.b * s.b + i * s.l + (p.hk * a.G + r - i * a.G) * s.h;
+      return (const T*)x + p.b * s.b + i * s.l + (p.hk * a.G + r - i * a.G) * s.h;
     };
-    sq.load(a.D, [&](int r) { return at(a.q, a.sq, r); });
-    sd.load(a.D, [&](int r) { return at(a.dout, a.sdo, r); });
-    rl = INFINITY, rd = 0.f;
-    const int r = r0 + threadIdx.x;
-    if (threadIdx.x < RB && r < a.M) {
-      const int i = row_pos(a, r);
-      const long long x = ((long long)p.b * a.Hq + p.hk * a.G + r - i * a.G) * a.Lq + i;
-      rl = a.lse[x] * LOG2E, rd = a.delta[x];
-      if (rl == -INFINITY) rl = INFINITY;
+    Dm::rows([&](int r) { return at(a.q, a.sq, r); }, a.D, base + buf * F::STAGE, wave, lane);
+    Dm::rows([&](int r) { return at(a.dout, a.sdo, r); }, a.D, base + buf * F::STAGE + F::TILE, wave, lane);
+    if (wave < 2) {
+      const int r = r0 + lane;
+      if (lane < RB) {
+        const int rr = min(r, a.M - 1), i = row_pos(a, rr);
+        const long long x = ((long long)p.b * a.Hq + p.hk * a.G + rr - i * a.G) * a.Lq + i;
+        const float* src = wave ? (r < a.M ? a.delta + x : (const float*)attn_zero) : (r < a.M ? a.lse2 + x : &attn_inf);
+        dma4(src, base + F::stats_at + buf * 512 + wave * 256);
+      }
     }
-  };
-  const auto put = [&](int buf) {
-    sq.store(qs + buf * RB * LQ, LQ), sd.store(ds + buf * RB * LQ, LQ);
-    if (threadIdx.x < RB) ls[buf * RB + threadIdx.x] = rl, ls[(2 + buf) * RB + threadIdx.x] = rd;
   };
 
   for (int half = 0; half < (a.causal ? 2 : 1); ++half) {
     const int tile = half ? a.tiles - 1 - tu : tu;
     if (half && tile <= tu) break;
     if (half) __syncthreads();  // the join of the first tile has been read
+    if ((half == 0 || WR > 1) && a.D * (int)sizeof(T) < L::ROWB) clear_lds(attn_smem, (int)F::stage_bytes, F::NTH);
     const int j0 = tile * BN, key = j0 + wn * TM + n;
     const bool seen = key < p.len && (!km || km[key]);
     // first row that sees the lane's key / the wave's first key / all of the wave's keys
     const int rmin = first_row(key), rany = first_row(j0 + wn * TM), rall = first_row(j0 + wn * TM + TM - 1);
-    int rbeg = j0 < p.len ? first_row(j0) : INT_MAX, rend = rbeg;
+    int rbeg = j0 < p.len ? first_row(j0) : INT_MAX, rend;
     if (rbeg < a.M) {
       const int b0 = rbeg / RB, blocks = (a.M + RB - 1) / RB - b0;
       rbeg = (b0 + (int)((long long)blocks * split / a.nsplit)) * RB;
       rend = min((b0 + (int)((long long)blocks * (split + 1) / a.nsplit)) * RB, a.M);
+    } else {
+      rbeg = rend = 0;  // no row sees a key of the tile
     }
 
     typename M::Frag kf[KF], vf[VL ? 1 : KF];
     load_frags<T, KF>(kf, seen ? (const T*)a.k + p.b * a.sk.b + key * a.sk.l + p.hk * a.sk.h : nullptr, a.D, h);
     if constexpr (VL) {
-      Stage<T, DP, BN, NTH> sv;
-      sv.load(a.D, [&](int j) {
-        return j0 + j < p.len && (!km || km[j0 + j]) ? (const T*)a.v + p.b * a.sv.b + (j0 + j) * a.sv.l + p.hk * a.sv.h
-                                                     : (const T*)nullptr;
-      });
-      sv.store(vs, LV);
+      Dma<T, DP, BN, NW>::rows(
+          [&](int j) {
+            return j0 + j < p.len && (!km || km[j0 + j]) ? (const T*)a.v + p.b * a.sv.b + (j0 + j) * a.sv.l + p.hk * a.sv.h
+                                                         : (const T*)nullptr;
+          },
+          a.D, base + F::v_at, wave, lane);
     } else {
       load_frags<T, KF>(vf, seen ? (const T*)a.v + p.b * a.sv.b + key * a.sv.l + p.hk * a.sv.h : nullptr, a.D, h);
     }
-    const T* vw = vs + wn * TM * LV;
 
     typename M::Acc dk[MD], dv[MD];
 #pragma unroll
     for (int md = 0; md < MD; ++md) dk[md] = dv[md] = (typename M::Acc)(0.f);
-    if (rbeg < rend) {
-      request(rbeg);
-      put(0);
-      if (rbeg + RB < rend) request(rbeg + RB);
-      __syncthreads();
-    }
+    if (rbeg < rend) request(rbeg, 0);
+    if (rbeg + RB < rend) request(rbeg + RB, 1);
+    stage_done<0, true>();
     int buf = 0;
-    for (int r0 = rbeg; r0 < rend; r0 += RB, buf ^= 1) {
-      if (r0 + RB < rend) {
-        put(buf ^ 1);
-        if (r0 + 2 * RB < rend) request(r0 + 2 * RB);
-      }
+    for (int r0 = rbeg; r0 < rend; r0 += RB) {
+      const bool more = r0 + 2 * RB < rend;
+      if (more) request(r0 + 2 * RB, buf == 0 ? 2 : buf - 1);
       const int rw = r0 + wr * F::RW;
       if (rw + F::RW > rany) {
         const bool partly = rw < rall;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          const int lr = buf * RB + wr * F::RW + mt * TM;  // the tile's row in LDS
-          const T* qt = qs + lr * LQ;
-          const T* dt = ds + lr * LQ;
+          const int lr = wr * F::RW + mt * TM;  // the tile's row in the stage
+          const char* qt = attn_smem + buf * F::STAGE + lr * L::ROWB;
+          const char* dt = qt + F::TILE;
           typename M::Acc sc = (typename M::Acc)(0.f), dp = (typename M::Acc)(0.f);
 #pragma unroll
           for (int f = 0; f < KF; ++f) {
-            sc = M::mma(rowfrag<T>(qt + 16 * f, LQ, lane), kf[f], sc);
-            if constexpr (VL) dp = M::mma(rowfrag<T>(dt + 16 * f, LQ, lane), rowfrag<T>(vw + 16 * f, LV, lane), dp);
-            else dp = M::mma(rowfrag<T>(dt + 16 * f, LQ, lane), vf[f], dp);
+            sc = M::mma(L::rowfrag(qt, f, lane), kf[f], sc);
+            if constexpr (VL) dp = M::mma(L::rowfrag(dt, f, lane), L::rowfrag(vw, f, lane), dp);
+            else dp = M::mma(L::rowfrag(dt, f, lane), vf[f], dp);
           }
+          const float* st = stats + buf * 128 + lr;
 #pragma unroll
           for (int q = 0; q < M::NC / 4; ++q) {
             const int r = M::crow(4 * q, h);
-            const fl4 l4 = *(const fl4*)(ls + lr + r), d4 = *(const fl4*)(ls + 2 * RB + lr + r);
+            const fl4 l4 = *(const fl4*)(st + r), d4 = *(const fl4*)(st + 64 + r);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float x = exp2_(__builtin_fmaf(sc[4 * q + e], a.c, -l4[e]));
@@ -724,13 +838,16 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) k_attn_dkv(const AttnP a) {
             const typename M::Frag pf = M::pack(sc, t), sf = M::pack(dp, t);
 #pragma unroll
             for (int md = 0; md < MD; ++md) {
-              dv[md] = M::mma(M::colfrag(dt + 16 * t * LQ + md * TM, LQ, lane), pf, dv[md]);
-              dk[md] = M::mma(M::colfrag(qt + 16 * t * LQ + md * TM, LQ, lane), sf, dk[md]);
+              dv[md] = M::mma(L::colfrag(dt + 16 * t * L::ROWB, md, lane), pf, dv[md]);
+              dk[md] = M::mma(L::colfrag(qt + 16 * t * L::ROWB, md, lane), sf, dk[md]);
             }
           }
         }
       }
-      __syncthreads();
+      // the next stage has landed; the one after it may be on its way
+      if (more) stage_done<F::LOADS, true>();
+      else stage_done<0, true>();
+      buf = buf == 2 ? 0 : buf + 1;
     }
     if constexpr (WR == 2) {  // wave 0 of a pair finishes dk, wave 1 finishes dv
       fl4* x = (fl4*)attn_smem + (wn * 2) * MD * (M::NC / 4) * 64 + lane;
@@ -755,7 +872,6 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) k_attn_dkv(const AttnP a) {
             for (int e = 0; e < 4; ++e) o[md][4 * q + e] += y[e];
           }
       };
-      if (rbeg >= rend) __syncthreads();  // no stage: the values' tile may still be on its way into the same memory
       if (wr) give(dk, 0);
       else give(dv, 1);
       __syncthreads();
@@ -811,7 +927,7 @@ int launch(K kernel, const char* name, long long grid, int threads, size_t lds, 
 
 // How a forward call is cut: rows per workgroup, keys per stage, splits of the keys.
 struct Plan {
-  bool few;  // few rows per problem: the waves of a workgroup share the rows and divide the keys
+  bool few;  // one tile of rows per problem: the waves of a workgroup share the rows and divide the keys
   int bm, tiles, nsplit, split_keys;
 };
 
@@ -890,13 +1006,13 @@ int forward_t(AttnP& a, const Plan& pl, hipStream_t st) {
   const long long grid = grid_of((long long)a.B * a.Hkv, (long long)pl.tiles * pl.nsplit);
   int rc;
   if (pl.few) {
-    constexpr int KT = F32 && DP > 64 ? 16 : 32;  // four waves' keys and values of a stage: at most 76 KB
-    using F = Fwd<T, DP, 1, 4, KT, 1>;
-    rc = launch(k_attn_fwd<T, DP, 1, 4, KT, 1>, "k_attn_fwd", grid, F::NTH, F::lds, st, a);
+    constexpr int KT = F32 && DP > 64 ? 16 : 32;  // two stages of four waves' keys and values: at most 128 KB
+    using F = Few<T, DP, 4, KT>;
+    rc = launch(k_attn_few<T, DP, 4, KT>, "k_attn_few", grid, F::NTH, F::lds, st, a);
   } else {
-    constexpr int NB = F32 && DP > 64 ? 1 : 2;
-    using F = Fwd<T, DP, 4, 1, 64, NB>;
-    rc = launch(k_attn_fwd<T, DP, 4, 1, 64, NB>, "k_attn_fwd", grid, F::NTH, F::lds, st, a);
+    constexpr int KT = F32 && DP > 64 ? 32 : 64;  // two stages of 64 KB at most: two workgroups per CU
+    using F = Fwd<T, DP, 4, KT>;
+    rc = launch(k_attn_fwd<T, DP, 4, KT>, "k_attn_fwd", grid, F::NTH, F::lds, st, a);
   }
   if (rc || pl.nsplit == 1) return rc;
   const long long rows = (long long)a.B * a.Hkv * a.M;
@@ -926,7 +1042,7 @@ int backward_t(AttnP& a, int nsplit, hipStream_t st) {
   const long long prob = (long long)a.B * a.Hkv;
   {
     constexpr int KT = F32 && DP > 64 ? 32 : 64;
-    using F = Dq<T, DP, 4, KT>;
+    using F = Fwd<T, DP, 4, KT>;
     a.tiles = (a.M + F::BM - 1) / F::BM;
     const int rc = launch(k_attn_dq<T, DP, 4, KT>, "k_attn_dq", grid_of(prob, a.tiles), F::NTH, F::lds, st, a);
     if (rc) return rc;
@@ -954,9 +1070,9 @@ int by_width(int D, Fn fn) {  // head widths are padded to the next of these wit
 extern "C" size_t gpn_attn_workspace_bytes(const gpn_attn_args_t* x, int backward) {
   if (check_args(x, "gpn_attn_workspace_bytes") || x->B == 0 || x->Lq == 0) return 0;
   const size_t rows = (size_t)x->B * x->Hq * x->Lq;
-  if (backward) {  // delta, and the parts of dk and dv
+  if (backward) {  // delta, log-sum-exp in powers of two, and the parts of dk and dv
     const int s = plan_dkv(x);
-    return align256(rows * 4) + (s > 1 ? (size_t)s * 2 * x->B * x->Lk * x->Hkv * x->D * 4 : 0);
+    return 2 * align256(rows * 4) + (s > 1 ? (size_t)s * 2 * x->B * x->Lk * x->Hkv * x->D * 4 : 0);
   }
   const Plan p = plan_forward(x);
   return p.nsplit == 1 ? 0 : align256(rows * p.nsplit * 4) + rows * p.nsplit * x->D * 4;
@@ -1015,7 +1131,9 @@ extern "C" int gpn_attn_backward(const gpn_attn_args_t* x, gpn_stream_t stream) 
   AttnP a = fill(x);
   const int nsplit = plan_dkv(x);
   a.delta = (float*)x->workspace;
-  a.part_o = (float*)((char*)x->workspace + align256((size_t)x->B * x->Hq * x->Lq * 4));
+  const size_t stat = align256((size_t)x->B * x->Hq * x->Lq * 4);
+  a.lse2 = (float*)((char*)x->workspace + stat);
+  a.part_o = (float*)((char*)x->workspace + 2 * stat);
   hipStream_t st = (hipStream_t)stream;
   return by_width(x->D, [&](auto dp) {
     return x->dtype == GPN_DT_F32 ? backward_t<float, decltype(dp)::value>(a, nsplit, st)
