@@ -950,9 +950,17 @@ __global__ void __launch_bounds__(64 * MB / Mt<T>::TM, 2) k_attn_short(const Att
     return j < p.len && (!km || km[j]) ? (const T*)x + p.b * s.b + j * s.l + p.hk * s.h : (const T*)nullptr;
   };
   using Dm = Dma<T, DP, MB, NW>;
-  Dm::rows([&](int r) { return r < a.M ? row_at(a.q, a.sq, r) : (const T*)nullptr; }, a.D, base + F::q_at, wave, lane);
-  Dm::rows([&](int r) { return r < a.M ? row_at(a.dout, a.sdo, r) : (const T*)nullptr; }, a.D, base + F::do_at, wave, lane);
-  Dm::rows([&](int j) { return key_at(a.k, a.sk, j); }, a.D, base + F::k_at, wave, lane);
+  if (a.G == 1 && a.M == MB && max(a.sq.l, a.sdo.l) < (1 << 22)) {
+    Dm::whole(row_at(a.q, a.sq, 0), a.sq.l, a.D, base + F::q_at, wave, lane);
+    Dm::whole(row_at(a.dout, a.sdo, 0), a.sdo.l, a.D, base + F::do_at, wave, lane);
+  } else {
+    Dm::rows([&](int r) { return r < a.M ? row_at(a.q, a.sq, r) : (const T*)nullptr; }, a.D, base + F::q_at, wave, lane);
+    Dm::rows([&](int r) { return r < a.M ? row_at(a.dout, a.sdo, r) : (const T*)nullptr; }, a.D, base + F::do_at, wave, lane);
+  }
+  if (!km && p.len == MB && a.sk.l < (1 << 22))
+    Dm::whole((const T*)a.k + p.b * a.sk.b + p.hk * a.sk.h, a.sk.l, a.D, base + F::k_at, wave, lane);
+  else
+    Dm::rows([&](int j) { return key_at(a.k, a.sk, j); }, a.D, base + F::k_at, wave, lane);
 
   // the wave's keys
   const int key = wave * TM + n;
@@ -990,51 +998,59 @@ __global__ void __launch_bounds__(64 * MB / Mt<T>::TM, 2) k_attn_short(const Att
   typename M::Acc dk[MD], dv[MD];
 #pragma unroll
   for (int md = 0; md < MD; ++md) dk[md] = dv[md] = (typename M::Acc)(0.f);
-  if (wave < ktiles) {
-    for (int r0 = 0; r0 < a.M; r0 += TM) {
-      typename M::Acc dp = (typename M::Acc)(0.f);
-      if (r0 + TM > rany) {
-        const char* qt = attn_smem + F::q_at + r0 * L::ROWB;
-        const char* dt = attn_smem + F::do_at + r0 * L::ROWB;
-        typename M::Acc sc = (typename M::Acc)(0.f);
+  // one tile of rows: its part of dv and dk, and ds -> LDS.  `partly`: some of the tile's rows do not see some of the keys.
+  const auto rows = [&](int r0, auto partly) {
+    const char* qt = attn_smem + F::q_at + r0 * L::ROWB;
+    const char* dt = attn_smem + F::do_at + r0 * L::ROWB;
+    typename M::Acc sc = (typename M::Acc)(0.f), dp = (typename M::Acc)(0.f);
 #pragma unroll
-        for (int f = 0; f < KF; ++f) {
-          sc = M::mma(L::rowfrag(qt, f, lane), kf[f], sc);
-          dp = M::mma(L::rowfrag(dt, f, lane), vf[f], dp);
-        }
-        const bool partly = r0 < rall || __any(!seen);
+    for (int f = 0; f < KF; ++f) {
+      sc = M::mma(L::rowfrag(qt, f, lane), kf[f], sc);
+      dp = M::mma(L::rowfrag(dt, f, lane), vf[f], dp);
+    }
 #pragma unroll
-        for (int q = 0; q < M::NC / 4; ++q) {
-          const int r = r0 + M::crow(4 * q, h);
-          const fl4 l4 = *(const fl4*)(st + r), d4 = *(const fl4*)(st + MB + r);
+    for (int q = 0; q < M::NC / 4; ++q) {
+      const int r = r0 + M::crow(4 * q, h);
+      const fl4 l4 = *(const fl4*)(st + r), d4 = *(const fl4*)(st + MB + r);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = exp2_(__builtin_fmaf(sc[4 * q + e], a.c, -l4[e]));
-            if (partly && (r + e < rmin || !seen)) x = 0.f;
-            sc[4 * q + e] = x;
-            dp[4 * q + e] = x * (dp[4 * q + e] - d4[e]);
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < TM / 16; ++t) {
-          const typename M::Frag pf = M::pack(sc, t), sf = M::pack(dp, t);
-#pragma unroll
-          for (int md = 0; md < MD; ++md) {
-            dv[md] = M::mma(L::colfrag(dt + 16 * t * L::ROWB, md, lane), pf, dv[md]);
-            dk[md] = M::mma(L::colfrag(qt + 16 * t * L::ROWB, md, lane), sf, dk[md]);
-          }
-        }
+      for (int e = 0; e < 4; ++e) {
+        float x = exp2_(__builtin_fmaf(sc[4 * q + e], a.c, -l4[e]));
+        if (decltype(partly)::value && (r + e < rmin || !seen)) x = 0.f;
+        sc[4 * q + e] = x;
+        dp[4 * q + e] = x * (dp[4 * q + e] - d4[e]);
       }
+    }
 #pragma unroll
-      for (int q = 0; q < M::NC / 4; ++q) {  // four neighbouring rows of the lane's key
-        typedef T V4 __attribute__((ext_vector_type(4)));
+    for (int t = 0; t < TM / 16; ++t) {
+      const typename M::Frag pf = M::pack(sc, t), sf = M::pack(dp, t);
+#pragma unroll
+      for (int md = 0; md < MD; ++md) {
+        dv[md] = M::mma(L::colfrag(dt + 16 * t * L::ROWB, md, lane), pf, dv[md]);
+        dk[md] = M::mma(L::colfrag(qt + 16 * t * L::ROWB, md, lane), sf, dk[md]);
+      }
+      typedef T V4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+      for (int g = 0; g < M::EP / 4; ++g) {  // four neighbouring rows of the lane's key
         V4 y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = (T)dp[4 * q + e];
-        const int at = (r0 + M::crow(4 * q, h)) * (int)sizeof(T);
+        for (int e = 0; e < 4; ++e) y[e] = sf[4 * g + e];
+        const int at = (r0 + M::crow(M::EP * t + 4 * g, h)) * (int)sizeof(T);
         *(V4*)(xs + xp * X::ROWB + ((at >> 4 ^ xw) << 4) + (at & 15)) = y;
       }
     }
+  };
+  if (wave < ktiles) {
+    const bool hidden = __any(!seen);
+    int r0 = 0;
+    for (; r0 < a.M && r0 + TM <= rany; r0 += TM) {  // rows before the first that sees a key of the wave: ds is zero
+#pragma unroll
+      for (int x = 0; x < TM * TM * (int)sizeof(T) / 1024; ++x) {
+        const int kx = wave * TM + lane % TM, at = r0 * (int)sizeof(T) + ((lane / TM) + x * (64 / TM)) * 16, px = X::phys(kx);
+        *(u4v*)(xs + px * X::ROWB + ((at >> 4 ^ X::swz(px)) << 4)) = u4v{0, 0, 0, 0};
+      }
+    }
+    for (; r0 < a.M && (hidden || r0 < rall); r0 += TM) rows(r0, std::true_type());
+    for (; r0 < a.M; r0 += TM) rows(r0, std::false_type());
   }
   if (key < a.Lk) {
     const long long at = (((long long)p.b * a.Lk + key) * a.Hkv + p.hk) * a.D;
