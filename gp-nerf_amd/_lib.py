@@ -5,6 +5,7 @@ call raises.  Tensors stay owned by PyTorch; kernels are enqueued on torch's cur
 """
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -104,6 +105,19 @@ class DistillArgs(C.Structure):
                 ("dlogits", C.c_void_p), ("drow_stride", C.c_longlong), ("dclass_stride", C.c_longlong)]
 
 
+def _packer(cls):
+    """struct.Struct with the layout of a ctypes mirror (arrays flattened, null pointers 0): filling a ctypes structure field by
+    field costs several microseconds, which a call of a few microseconds on the device would wait for."""
+    code = {C.c_int: "i", C.c_float: "f", C.c_longlong: "q", C.c_void_p: "P", C.c_size_t: "N"}
+    fmt = "@" + "".join(code[t] if t in code else "%d%s" % (t._length_, code[t._type_]) for _, t in cls._fields_)
+    s = struct.Struct(fmt)
+    assert s.size == C.sizeof(cls), cls.__name__
+    return s
+
+
+ATTN = _packer(AttnArgs)
+DISTILL = _packer(DistillArgs)
+
 _P = C.c_void_p
 _SIGS = {
     "gpn_abi_version": (C.c_int, []),
@@ -143,12 +157,12 @@ _SIGS = {
                                   C.POINTER(SemArgs), _P, _P, _P, _P, C.c_size_t, _P]),
     "gpn_gnt_forward_static": (C.c_int, [C.POINTER(GntWeights), _P, C.c_int, _P, _P, _P, _P, _P, C.c_int,
                                          C.c_int, C.c_int, C.POINTER(SemArgs), _P, _P, _P, _P]),
-    "gpn_attn_workspace_bytes": (C.c_size_t, [C.POINTER(AttnArgs), C.c_int]),
-    "gpn_attn_forward": (C.c_int, [C.POINTER(AttnArgs), _P]),
-    "gpn_attn_backward": (C.c_int, [C.POINTER(AttnArgs), _P]),
-    "gpn_distill_forward": (C.c_int, [C.POINTER(DistillArgs), _P]),
-    "gpn_distill_backward": (C.c_int, [C.POINTER(DistillArgs), _P]),
-    "gpn_distill_step": (C.c_int, [C.POINTER(DistillArgs), _P]),
+    "gpn_attn_workspace_bytes": (C.c_size_t, [_P, C.c_int]),
+    "gpn_attn_forward": (C.c_int, [_P, _P]),
+    "gpn_attn_backward": (C.c_int, [_P, _P]),
+    "gpn_distill_forward": (C.c_int, [_P, _P]),
+    "gpn_distill_backward": (C.c_int, [_P, _P]),
+    "gpn_distill_step": (C.c_int, [_P, _P]),
     "gpn_timing_begin": (C.c_int, [C.c_uint, C.c_int]),
     "gpn_timing_end": (C.c_int, [C.POINTER(C.c_double), C.POINTER(C.c_longlong)]),
 }
@@ -186,6 +200,18 @@ def check(code, what):
 
 def stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def call_on(dev, fn, name, args):
+    """fn(args, stream) on the current stream of `dev`, which need not be the current device."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        code = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    if code != 0:
+        check(code, name)
 
 
 def dev_f32(t, name, shape=None):

@@ -20,7 +20,6 @@ A key is visible to a query where all of these hold:
 A query that sees no key has out = 0, lse = -inf and no gradient.  Keys hidden by lengths or key_mask are never read: padding
 may hold anything.  Keys hidden by causal alone have to be finite, and so have the padding rows of q and dout.
 """
-import ctypes as C
 import math
 
 import torch
@@ -36,11 +35,15 @@ def _rows(t):
     for copy in (None, torch.Tensor.contiguous, torch.Tensor.clone):
         if copy is not None:
             t = copy(t)
-        s = t.stride()
-        n = t.shape
-        st = (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
-        if s[3] == 1 and t.data_ptr() % 16 == 0 and not (st[0] % per or st[1] % per or st[2] % per):
-            return t, st
+        sb, sl, sh, sd = t.stride()
+        if t.shape[0] < 2:
+            sb = 0
+        if t.shape[1] < 2:
+            sl = 0
+        if t.shape[2] < 2:
+            sh = 0
+        if sd == 1 and t.data_ptr() % 16 == 0 and not (sb % per or sl % per or sh % per):
+            return t, (sb, sl, sh)
     raise AssertionError("unreachable: a clone is aligned")
 
 
@@ -51,92 +54,86 @@ def _index(t, name, B, dev):
 
 
 def _args(q, k, v, lengths, key_mask, causal, q_start, scale):
-    """Checks what both directions take -> (gpn_attn_args_t without outputs, tensors that have to live until the launch)."""
-    _lib.dev_float(q, "q")
-    _lib.dev_float(k, "k", dtype=q.dtype)
-    _lib.dev_float(v, "v", dtype=q.dtype)
+    """Checks what both directions take -> (first part of the packed gpn_attn_args_t, up to q_start; its sizes; tensors that
+    have to live until the launch)."""
+    dt = _lib.dev_float(q, "q").dtype
+    _lib.dev_float(k, "k", None, dt)
+    _lib.dev_float(v, "v", None, dt)
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError("q must be [B, Lq, Hq, D] and k [B, Lk, Hkv, D]")
     B, Lq, Hq, D = q.shape
-    Lk, Hkv = k.shape[1], k.shape[2]
-    if k.shape[0] != B or k.shape[3] != D or v.shape != k.shape:
+    Bk, Lk, Hkv, Dk = k.shape
+    if Bk != B or Dk != D or v.shape != k.shape:
         raise ValueError("k and v must be [%d, Lk, Hkv, %d] (got %s and %s)" % (B, D, tuple(k.shape), tuple(v.shape)))
     if D % 8 or not 8 <= D <= MAX_D:
         raise ValueError("head width must be a multiple of 8 up to %d (got %d)" % (MAX_D, D))
     if Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise ValueError("%d query heads cannot share %d key/value heads" % (Hq, Hkv))
-    _lib.same_device(q, k=k, v=v)
+    dev = q.device
+    if k.device != dev or v.device != dev:
+        _lib.same_device(q, k=k, v=v)
     if q_start is not None and not causal:
         raise ValueError("q_start: only causal attention has positions")
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
     q, sq = _rows(q)
     k, sk = _rows(k)
     v, sv = _rows(v)
-    a = _lib.AttnArgs(_lib.DTYPES[q.dtype], B, Lq, Lk, Hq, Hkv, D, 1 if causal else 0, scale, q.data_ptr(), k.data_ptr(),
-                      v.data_ptr(), sq, sk, sv)
-    keep = [q, k, v]
     if lengths is not None:
-        lengths = _index(lengths, "lengths", B, q.device)
-        a.lengths = lengths.data_ptr()
-        keep.append(lengths)
+        lengths = _index(lengths, "lengths", B, dev)
     if q_start is not None:
-        q_start = _index(q_start, "q_start", B, q.device)
-        a.q_start = q_start.data_ptr()
-        keep.append(q_start)
+        q_start = _index(q_start, "q_start", B, dev)
     if key_mask is not None:
         if not isinstance(key_mask, torch.Tensor) or key_mask.dtype not in (torch.bool, torch.uint8) or \
-                tuple(key_mask.shape) != (B, Lk) or key_mask.device != q.device:
-            raise ValueError("key_mask: expected a bool or uint8 tensor of shape (%d, %d) on %s" % (B, Lk, q.device))
+                tuple(key_mask.shape) != (B, Lk) or key_mask.device != dev:
+            raise ValueError("key_mask: expected a bool or uint8 tensor of shape (%d, %d) on %s" % (B, Lk, dev))
         if Lk > 1 and key_mask.stride(1) != 1:
             key_mask = key_mask.contiguous()
-        a.key_mask, a.key_mask_stride = key_mask.data_ptr(), key_mask.stride(0)
-        keep.append(key_mask)
-    return a, keep
+    head = (_lib.DTYPES[dt], B, Lq, Lk, Hq, Hkv, D, 1 if causal else 0, 1.0 / math.sqrt(D) if scale is None else scale,
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), *sq, *sk, *sv, 0 if lengths is None else lengths.data_ptr(),
+            0 if key_mask is None else key_mask.data_ptr(), 0 if key_mask is None else key_mask.stride(0),
+            0 if q_start is None else q_start.data_ptr())
+    return head, (q, k, v, lengths, q_start, key_mask)
 
 
-def _call(a, backward, dev):
+def _call(fn, name, backward, dev, *fields):
     """Workspace and launch on the current stream of the tensors' device."""
-    L = _lib.lib()
-    with torch.cuda.device(dev):
-        need = L.gpn_attn_workspace_bytes(C.byref(a), backward)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        if need:
-            a.workspace, a.workspace_bytes = ws.data_ptr(), need
-        fn, name = (L.gpn_attn_backward, "gpn_attn_backward") if backward else (L.gpn_attn_forward, "gpn_attn_forward")
-        _lib.check(fn(C.byref(a), _lib.stream()), name)
+    pack = _lib.ATTN.pack
+    args = pack(*fields, 0, 0)
+    need = _lib.lib().gpn_attn_workspace_bytes(args, backward)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        args = pack(*fields, ws.data_ptr(), need)
+    _lib.call_on(dev, fn, name, args)
 
 
-@torch.no_grad()
 def attention_forward(q, k, v, lengths=None, key_mask=None, causal=False, q_start=None, scale=None):
     """-> out [B, Lq, Hq, D] of q's type, lse [B, Hq, Lq] float32 (natural logarithm of the row's sum; -inf without a key).
-    scale: of the scores, positive (1 / sqrt(D) unless given)."""
-    a, keep = _args(q, k, v, lengths, key_mask, causal, q_start, scale)
+    scale: of the scores, positive (1 / sqrt(D) unless given).  No graph is recorded."""
+    head, keep = _args(q, k, v, lengths, key_mask, causal, q_start, scale)
     B, Lq, Hq, D = q.shape
-    out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=q.device)
-    a.out, a.lse = out.data_ptr(), lse.data_ptr()
-    _call(a, 0, q.device)
+    dev = q.device
+    out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=dev)
+    _call(_lib.lib().gpn_attn_forward, "gpn_attn_forward", 0, dev, *head, out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0, 0, 0)
     return out, lse
 
 
-@torch.no_grad()
 def attention_backward(dout, q, k, v, out, lse, lengths=None, key_mask=None, causal=False, q_start=None, scale=None):
     """Gradients of sum(out * dout) -> dq, dk, dv (shapes and type of q, k, v, contiguous).  out and lse are what
-    attention_forward returned for the same arguments; the probabilities are computed again from them."""
-    a, keep = _args(q, k, v, lengths, key_mask, causal, q_start, scale)
-    B, Lq, Hq, D = q.shape
-    _lib.dev_float(dout, "dout", (B, Lq, Hq, D), q.dtype)
-    _lib.dev_float(out, "out", (B, Lq, Hq, D), q.dtype)
-    _lib.dev_float(lse, "lse", (B, Hq, Lq), torch.float32)
-    _lib.same_device(q, dout=dout, out=out, lse=lse)
+    attention_forward returned for the same arguments; the probabilities are computed again from them.  No graph is recorded."""
+    head, keep = _args(q, k, v, lengths, key_mask, causal, q_start, scale)
+    shape, dt, dev = q.shape, q.dtype, q.device
+    _lib.dev_float(dout, "dout", shape, dt)
+    _lib.dev_float(out, "out", shape, dt)
+    _lib.dev_float(lse, "lse", (shape[0], shape[2], shape[1]), torch.float32)
+    if dout.device != dev or out.device != dev or lse.device != dev:
+        _lib.same_device(q, dout=dout, out=out, lse=lse)
     dout, sdo = _rows(dout)
-    out = out if out.is_contiguous() and out.data_ptr() % 16 == 0 else out.clone(memory_format=torch.contiguous_format)
+    if not out.is_contiguous() or out.data_ptr() % 16:
+        out = out.clone(memory_format=torch.contiguous_format)
     lse = lse.contiguous()
-    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
-    a.out, a.lse, a.dout, a.dout_stride = out.data_ptr(), lse.data_ptr(), dout.data_ptr(), sdo
-    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    _call(a, 1, q.device)
+    dq, dk, dv = (torch.empty(t.shape, dtype=dt, device=dev) for t in (q, k, v))
+    _call(_lib.lib().gpn_attn_backward, "gpn_attn_backward", 1, dev, *head, out.data_ptr(), lse.data_ptr(), dout.data_ptr(), *sdo,
+          dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
     return dq, dk, dv
 
 

@@ -59,14 +59,15 @@ def _as_rows(x, name):
     raise ValueError("%s: expected [N, classes], [classes, H, W] or [1, classes, H, W]" % name)
 
 
-def _distill_args(logits, teacher_logits, teacher_index, temperature, row_weight, reduction):
-    """Checks -> (gpn_distill_args_t, logits as rows, tensors that have to live until the launch)."""
+def _distill_args(logits, teacher_logits, teacher_index, temperature, row_weight, reduction, grad_scale=1.0):
+    """Checks -> (first part of the packed gpn_distill_args_t, up to row_weight; logits as rows; whether their rows are what is
+    contiguous; tensors that have to live until the launch)."""
     z = _lib.dev_float(_as_rows(logits, "logits"), "logits")
     t = _lib.dev_float(_as_rows(teacher_logits, "teacher_logits"), "teacher_logits")
     x = _as_rows(teacher_index, "teacher_index")
     N, Cn = z.shape
     K = t.shape[1]
-    if t.shape[0] != N or tuple(x.shape) != (N, K):
+    if t.shape[0] != N or x.shape != t.shape:
         raise ValueError("teacher_logits and teacher_index must have a row of K entries for each of the %d rows (got %s and %s)"
                          % (N, tuple(t.shape), tuple(x.shape)))
     if x.dtype not in (torch.int32, torch.int64):
@@ -79,48 +80,34 @@ def _distill_args(logits, teacher_logits, teacher_index, temperature, row_weight
         raise ValueError("reduction must be one of %s (got %r)" % (sorted(_REDUCTIONS), reduction))
     if row_weight is not None:
         row_weight = _lib.dev_float(row_weight, "row_weight", (N,), torch.float32).contiguous()
-    _lib.same_device(z, teacher_logits=t, teacher_index=x, row_weight=row_weight)
+    dev = z.device
+    if t.device != dev or x.device != dev or row_weight is not None:
+        _lib.same_device(z, teacher_logits=t, teacher_index=x, row_weight=row_weight)
     rs, cs = z.stride()
     planes = cs != 1 and Cn > 1
-    if planes and (rs != 1 and N > 1):
+    if planes and rs != 1 and N > 1:
         z = z.contiguous()
         (rs, cs), planes = z.stride(), False
-    a = _lib.DistillArgs(_lib.DTYPES[z.dtype], _lib.DTYPES[t.dtype], x.element_size(), Cn, K, _REDUCTIONS[reduction],
-                         temperature, 1.0, N, z.data_ptr(), rs, cs, t.data_ptr(), t.stride(), x.data_ptr(), x.stride())
-    if row_weight is not None:
-        a.row_weight = row_weight.data_ptr()
-    return a, z, planes, (z, t, x, row_weight)
+    head = (_lib.DTYPES[z.dtype], _lib.DTYPES[t.dtype], x.element_size(), Cn, K, _REDUCTIONS[reduction], temperature, grad_scale, N,
+            z.data_ptr(), rs, cs, t.data_ptr(), *t.stride(), x.data_ptr(), *x.stride(),
+            0 if row_weight is None else row_weight.data_ptr())
+    return head, z, planes, (t, x, row_weight)
 
 
-def _distill_outputs(a, z, loss, lse):
-    """Allocates the forward's outputs in one block -> (loss [] or [N], lse [N] or None)."""
-    N = z.shape[0]
-    rows = torch.empty(((1 + lse) * N + 1,), device=z.device)
-    a.loss_rows = rows.data_ptr()
-    a.loss = rows.data_ptr() + 4 * (1 + lse) * N
-    if lse:
-        a.lse = rows.data_ptr() + 4 * N
-    return (rows[:N] if loss == "none" else rows[-1]), (rows[N:2 * N] if lse else None)
-
-
-def _distill_gradient(a, z, planes, logits):
-    """Allocates dlogits as the logits lie (class planes or rows) -> it, in the logits' shape."""
+def _distill_gradient(z, planes, logits):
+    """Memory for dlogits as the logits lie (class planes or rows) -> it in the logits' shape, (address, strides)."""
     N, Cn = z.shape
     if planes:
         d = torch.empty((Cn, N), dtype=z.dtype, device=z.device)
-        a.dlogits, a.drow_stride, a.dclass_stride = d.data_ptr(), 1, N
-        return d.t() if logits.dim() == 2 else d.view(logits.shape)
+        return d.t() if logits.dim() == 2 else d.view(logits.shape), (d.data_ptr(), 1, N)
     d = torch.empty((N, Cn), dtype=z.dtype, device=z.device)
-    a.dlogits, a.drow_stride, a.dclass_stride = d.data_ptr(), Cn, 1
-    return d if logits.dim() == 2 else d.t().reshape(logits.shape)
+    return d if logits.dim() == 2 else d.t().reshape(logits.shape), (d.data_ptr(), Cn, 1)
 
 
-def _distill_call(name, a, dev):
-    with torch.cuda.device(dev):
-        _lib.check(getattr(_lib.lib(), name)(C.byref(a), _lib.stream()), name)
+def _distill_call(name, dev, *fields):
+    _lib.call_on(dev, getattr(_lib.lib(), name), name, _lib.DISTILL.pack(*fields))
 
 
-@torch.no_grad()
 def distill_topk_forward(logits, teacher_logits, teacher_index, temperature=1.0, row_weight=None, reduction="mean"):
     """Loss of class logits against a teacher's top logits: per row T^2 * KL(softmax of the teacher's K entries at
     temperature T || softmax of all the student's classes at T).
@@ -129,39 +116,40 @@ def distill_topk_forward(logits, teacher_logits, teacher_index, temperature=1.0,
     NeRFSemSegFPNHead gives it; float32 or bfloat16.  teacher_logits, teacher_index [N, K] (or [1, K, H, W]): what
     `teacher.topk(K, dim=1)` returns; int32 or int64 classes; an entry outside [0, C) (-1) is left out and a row
     without an entry counts as zero.  row_weight [N] float32: weight of each row (0 leaves it out).  reduction: 'mean' over
-    all N rows, 'sum' or 'none'.  -> loss (scalar, or [N]), lse [N] (what distill_topk_backward needs)."""
-    a, z, _, keep = _distill_args(logits, teacher_logits, teacher_index, temperature, row_weight, reduction)
-    loss, lse = _distill_outputs(a, z, reduction, 1)
-    _distill_call("gpn_distill_forward", a, z.device)
+    all N rows, 'sum' or 'none'.  -> loss (scalar, or [N]), lse [N] (what distill_topk_backward needs).  No graph is recorded."""
+    head, z, _, keep = _distill_args(logits, teacher_logits, teacher_index, temperature, row_weight, reduction)
+    N, dev = z.shape[0], z.device
+    rows = torch.empty(N, device=dev)
+    lse = torch.empty(N, device=dev)
+    loss = rows if reduction == "none" else torch.empty((), device=dev)
+    _distill_call("gpn_distill_forward", dev, *head, rows.data_ptr(), loss.data_ptr(), lse.data_ptr(), 0, 0, 0, 0)
     return loss, lse
 
 
-@torch.no_grad()
 def distill_topk_backward(dloss, logits, teacher_logits, teacher_index, lse, temperature=1.0, row_weight=None,
                           reduction="mean"):
     """Gradient of the logits for the loss's gradient `dloss` (float32; scalar, or [N] for 'none'); other arguments as given
     to distill_topk_forward, lse as it returned.  -> dlogits, of the logits' type, shape and layout."""
-    a, z, planes, keep = _distill_args(logits, teacher_logits, teacher_index, temperature, row_weight, reduction)
+    head, z, planes, keep = _distill_args(logits, teacher_logits, teacher_index, temperature, row_weight, reduction)
     N = z.shape[0]
     dloss = _lib.dev_float(dloss, "dloss", (N,) if reduction == "none" else (), torch.float32).contiguous()
     lse = _lib.dev_float(lse, "lse", (N,), torch.float32).contiguous()
     _lib.same_device(z, dloss=dloss, lse=lse)
-    a.dloss, a.lse = dloss.data_ptr(), lse.data_ptr()
-    d = _distill_gradient(a, z, planes, logits)
-    _distill_call("gpn_distill_backward", a, z.device)
+    d, at = _distill_gradient(z, planes, logits)
+    _distill_call("gpn_distill_backward", z.device, *head, 0, 0, lse.data_ptr(), dloss.data_ptr(), *at)
     return d
 
 
-@torch.no_grad()
 def distill_topk_step(logits, teacher_logits, teacher_index, temperature=1.0, row_weight=None, reduction="mean",
                       grad_scale=1.0):
     """distill_topk_forward and the gradient of `grad_scale * loss` in one pass over the logits, for a training step that
     knows the loss's weight (with 'none': of the sum of the rows).  -> loss, dlogits."""
-    a, z, planes, keep = _distill_args(logits, teacher_logits, teacher_index, temperature, row_weight, reduction)
-    a.grad_scale = grad_scale
-    loss, _ = _distill_outputs(a, z, reduction, 0)
-    d = _distill_gradient(a, z, planes, logits)
-    _distill_call("gpn_distill_step", a, z.device)
+    head, z, planes, keep = _distill_args(logits, teacher_logits, teacher_index, temperature, row_weight, reduction, grad_scale)
+    dev = z.device
+    rows = torch.empty(z.shape[0], device=dev)
+    loss = rows if reduction == "none" else torch.empty((), device=dev)
+    d, at = _distill_gradient(z, planes, logits)
+    _distill_call("gpn_distill_step", dev, *head, rows.data_ptr(), loss.data_ptr(), 0, 0, *at)
     return loss, d
 
 

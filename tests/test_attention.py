@@ -102,8 +102,8 @@ def test_c_entry_refuses_missing_workspace_and_gradients():
     from gp_nerf_amd import _lib
     L = _lib.lib()
     assert L.gpn_attn_forward(None, None) == -1 and b"null arguments" in L.gpn_last_error()
-    assert L.gpn_attn_workspace_bytes(ctypes.byref(_fake()), 1) >= 2 * 8 * 4 * 4
-    assert L.gpn_attn_backward(ctypes.byref(_fake()), None) == -1 and b"workspace" in L.gpn_last_error()
+    assert L.gpn_attn_workspace_bytes(ctypes.byref(_fake(Lq=300, Lk=300)), 1) >= 2 * 300 * 4 * 4
+    assert L.gpn_attn_backward(ctypes.byref(_fake(Lq=300, Lk=300)), None) == -1 and b"workspace" in L.gpn_last_error()
     for n in ("dq", "dk", "dv", "dout"):
         assert L.gpn_attn_backward(ctypes.byref(_fake(**{n: None})), None) == -1
         assert ("null " + n).encode() in L.gpn_last_error()

@@ -356,6 +356,6 @@ def test_ray_attention_under_a_distilled_head():
     # chains of at most 64 + 16 + 48 + 48 + 64 + 21 sums before the loss and the like behind it, 2400 rows for a weight: fewer
     # than 3200 half steps of 2^-24, on values whose magnitudes sum to at most 4 times the largest result
     tol = 4 * 3200 * 2.0 ** -24
-    assert abs(float(got) - float(want)) <= tol * abs(float(want))
+    assert abs(float(got.detach()) - float(want.detach())) <= tol * abs(float(want.detach()))
     for a, b in zip(own, ref):
         assert float((a.grad.cpu().double() - b.grad).abs().max()) <= tol * float(b.grad.abs().max())
