@@ -29,7 +29,7 @@ struct DistP {
   const float *w, *dloss, *lse_in;
   float *loss_rows, *lse;
   long long N;
-  int C, K, t_f32, i_64, dloss_rows;
+  int C, K, t_f32, i_64, dloss_rows, loss_each;  // loss_each: loss_rows is an output (else workgroups may leave sums there)
   float T, c;        // temperature, log2(e) / T
   float grad_scale;  // of the upstream gradient (1 / N for a mean)
   float loss_scale;  // of the sum over the rows
@@ -53,13 +53,6 @@ struct El<float> {
     for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(unsigned, x[i]);
     return r;
   }
-  static __device__ __forceinline__ u4v gather(const float* p, int lo, int hi) {  // elements lo .. hi-1 of a chunk, others -inf
-    u4v r = {NEG, NEG, NEG, NEG};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i >= lo && i < hi) r[i] = __builtin_bit_cast(unsigned, p[i]);
-    return r;
-  }
 };
 template <>
 struct El<bfu> {
@@ -71,20 +64,11 @@ struct El<bfu> {
   static __device__ __forceinline__ float load(const bfu* p) { return bf2f(*p); }
   static __device__ __forceinline__ void store(bfu* p, float x) { *p = f2bf(x); }
   static __device__ __forceinline__ u4v pack(const float* x) {
-    u4v r;
+    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+    b8 r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = (unsigned)f2bf(x[2 * i]) | (unsigned)f2bf(x[2 * i + 1]) << 16;
-    return r;
-  }
-  static __device__ __forceinline__ u4v gather(const bfu* p, int lo, int hi) {
-    u4v r = {NEG, NEG, NEG, NEG};
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i >= lo && i < hi) {
-        const unsigned x = p[i];
-        r[i >> 1] = i & 1 ? (r[i >> 1] & 0xffffu) | x << 16 : (r[i >> 1] & 0xffff0000u) | x;
-      }
-    return r;
+    for (int i = 0; i < 8; ++i) r[i] = (__bf16)x[i];
+    return __builtin_bit_cast(u4v, r);
   }
 };
 
@@ -118,37 +102,42 @@ __device__ __forceinline__ float row_factor(const DistP& a, long long row) {
 }
 
 // ---------------------------------------------------------------------------------------------------------- rows
-// NT threads, CH 16-byte chunks of the row in each thread's registers; a row of more than NT * CH chunks is walked in segments
-// and read again for the gradient.
-template <typename T, int NT, int CH, int MODE>
-__global__ void __launch_bounds__(NT) k_distill_rows(const DistP a) {
+// NT threads, CH 16-byte chunks of the row in each thread's registers.  MANY: a row of more than NT * CH chunks is walked in
+// segments and read again for the gradient.  The elements before the first and behind the last 16-byte boundary of the row
+// belong to the first 2 EP threads, one each.
+template <typename T, int NT, int CH, bool MANY, int MODE>
+__global__ void __launch_bounds__(NT, CH > 8 ? 4 : 6) k_distill_rows(const DistP a) {
   using E = El<T>;
   constexpr int EP = E::EP, NW = NT / 64;
-  __shared__ float sp[GPN_DISTILL_MAX_K], sred[2 * NW], sstat[4];
+  __shared__ float sp[GPN_DISTILL_MAX_K], sred[2 * NW], sstat[2];
   __shared__ int si[GPN_DISTILL_MAX_K];
   const long long row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const T* z = (const T*)a.z + row * a.z_rs;
   const int a0 = (int)(((size_t)z & 15) / sizeof(T));  // elements of the first chunk before the row
-  const int nch = (int)(((long long)a0 + a.C + EP - 1) / EP);
-  const T* zc = z - a0;
+  const int head = min(a0 ? EP - a0 : 0, a.C), nch = (a.C - head) / EP;  // then nch whole chunks from zc
+  const T* zc = z + head;
+  // the thread's own element at an end of the row (or none): head elements, then those behind the last chunk
+  const int edge = tid < head ? tid : tid >= EP && tid < 2 * EP && head + nch * EP + tid - EP < a.C ? head + nch * EP + tid - EP : -1;
+  const float xe = edge >= 0 ? E::load(z + edge) : -INFINITY;
 
   u4v r[CH];
+  int at = tid;  // opaque below: addresses are formed again for every pass rather than held over it
   const auto load = [&](int c0) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int c = c0 + tid + i * NT;
+      const int c = c0 + at + i * NT;
       r[i] = u4v{E::NEG, E::NEG, E::NEG, E::NEG};
-      if (c < nch) {
-        const long long e = (long long)c * EP;
-        const int lo = c == 0 ? a0 : 0;
-        const long long left = a.C + a0 - e;
-        if (lo == 0 && left >= EP) r[i] = *(const u4v*)(zc + e);
-        else r[i] = E::gather(zc + e, lo, left < EP ? (int)left : EP);
-      }
+      if (c < nch) r[i] = *(const u4v*)((const char*)zc + (unsigned)c * 16u);
     }
   };
-  const int seg = NT * CH;
+  // unpack again rather than hold the row a second time, in fp32
+  const auto again = [&]() {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) asm volatile("" : "+v"(r[i]));
+    asm volatile("" : "+v"(at));
+  };
+  constexpr int seg = NT * CH;
   load(0);
 
   // teacher: wave 0 walks the K entries while the row is on its way
@@ -158,32 +147,36 @@ __global__ void __launch_bounds__(NT) k_distill_rows(const DistP a) {
       const int x = entry_class(a, row, k);
       const float t = x >= 0 ? entry_logit(a, row, k) : -INFINITY;
       si[k] = x, sp[k] = t;
-      const float M = fmaxf(mt, t), s = base_of(M);
-      lt = lt * exp2_((mt - s) * a.c) + exp2_((t - s) * a.c);
-      mt = M;
+      merge(mt, lt, t, 1.f, a.c);
     }
 #pragma unroll
     for (int d = 32; d; d >>= 1) merge(mt, lt, __shfl_xor(mt, d), __shfl_xor(lt, d), a.c);
     if (lane == 0) sstat[0] = mt, sstat[1] = lt;
   }
 
-  float m = -INFINITY, l = 0.f;
+  // log2 of a logit's probability: (x - m) c - l2.  The difference comes first: x c - m c of logits of 10^9 would be noise.
+  float m = xe, l = fabsf(xe) == INFINITY ? exp2_(xe) : edge >= 0 ? exp2_((xe - base_of(xe)) * a.c) : 0.f;
   if (MODE != BWD) {
     for (int c0 = 0;;) {
       float mx = m;
 #pragma unroll
       for (int i = 0; i < CH; ++i)
+        if (c0 + i * NT < nch) {
 #pragma unroll
-        for (int e = 0; e < EP; ++e) mx = fmaxf(mx, E::get(r[i], e));
-      const float s = base_of(mx);
-      l *= exp2_((m - s) * a.c);
+          for (int e = 0; e < EP; ++e) mx = fmaxf(mx, E::get(r[i], e));
+        }
+      const float b = base_of(mx);
+      l *= exp2_((m - b) * a.c);
       m = mx;
+      again();
 #pragma unroll
       for (int i = 0; i < CH; ++i)
+        if (c0 + i * NT < nch) {
 #pragma unroll
-        for (int e = 0; e < EP; ++e) l += exp2_((E::get(r[i], e) - s) * a.c);
+          for (int e = 0; e < EP; ++e) l += exp2_((E::get(r[i], e) - b) * a.c);
+        }
       c0 += seg;
-      if (c0 >= nch) break;
+      if (!MANY || c0 >= nch) break;
       load(c0);
     }
 #pragma unroll
@@ -199,7 +192,6 @@ __global__ void __launch_bounds__(NT) k_distill_rows(const DistP a) {
   const float mt = sstat[0], lt = sstat[1];
   const bool empty = !(lt > 0.f) && lt == lt;  // no entry at all
   const float lt2 = log2_(lt);
-  // log2 of the student's probability of a logit x: (x - m) c - l2
   float l2;
   if (MODE == BWD) m = 0.f, l2 = a.lse_in[row] * LOG2E;
   else l2 = log2_(l);
@@ -220,36 +212,42 @@ __global__ void __launch_bounds__(NT) k_distill_rows(const DistP a) {
   if (MODE == FWD) return;
 
   const float f = row_factor(a, row);
+  const float inv = MODE == BWD ? 0.f : 1.f / l, fi = f * inv;
+  const auto prob = [&](float x) {
+    const float u = (x - m) * a.c;
+    return MODE == BWD ? exp2_(u - l2) : exp2_(u) * inv;
+  };
   T* dz = (T*)a.dz + row * a.d_rs;
+  if (empty) {  // zero whatever the logits hold
+    for (int c = tid; c < a.C; c += NT) E::store(dz + c, 0.f);
+    return;
+  }
+  const auto grad = [&](float x) {
+    const float u = (x - m) * a.c;
+    return MODE == BWD ? f * exp2_(u - l2) : fi * exp2_(u);
+  };
+  if (edge >= 0) E::store(dz + edge, grad(xe));
   const bool same = (((size_t)dz ^ (size_t)z) & 15) == 0;  // 16-byte stores meet 16-byte loads
-  const float inv = MODE == BWD ? 0.f : 1.f / l;
   for (int c0 = 0; c0 < nch; c0 += seg) {
-    if (nch > seg && (MODE == BWD ? c0 > 0 : true)) load(c0);
+    again();
+    if (MANY && (MODE == BWD ? c0 > 0 : true)) load(c0);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int c = c0 + tid + i * NT;
+      const int c = c0 + at + i * NT;
       if (c < nch) {
         float y[EP];
 #pragma unroll
-        for (int e = 0; e < EP; ++e) {
-          const float x = (E::get(r[i], e) - m) * a.c;
-          const float s = MODE == BWD ? exp2_(x - l2) : exp2_(x) * inv;
-          y[e] = empty ? 0.f : f * s;
-        }
-        const long long at = (long long)c * EP - a0;
-        const int lo = c == 0 ? a0 : 0;
-        const long long left = a.C - at;
-        if (same && lo == 0 && left >= EP) {
-          *(u4v*)(dz + at) = E::pack(y);
+        for (int e = 0; e < EP; ++e) y[e] = grad(E::get(r[i], e));
+        T* d = (T*)((char*)(dz + head) + (unsigned)c * 16u);
+        if (same) {
+          *(u4v*)d = E::pack(y);
         } else {
 #pragma unroll
-          for (int e = 0; e < EP; ++e)
-            if (e >= lo && e < left) E::store(dz + at + e, y[e]);
+          for (int e = 0; e < EP; ++e) E::store(d + e, y[e]);
         }
       }
     }
   }
-  if (empty) return;
   // The teacher's classes: their entries are written a second time, behind the barrier.  A class that stands in the row twice
   // has both probabilities in its sum, in the order of the entries, whichever of the two writes it.
   __threadfence_block();
@@ -260,93 +258,230 @@ __global__ void __launch_bounds__(NT) k_distill_rows(const DistP a) {
     float p = 0.f;
     for (int j = 0; j < a.K; ++j)
       if (si[j] == x) p += exp2_((sp[j] - mt) * a.c - lt2);
-    const float u = (E::load(z + x) - m) * a.c, s = MODE == BWD ? exp2_(u - l2) : exp2_(u) * inv;
-    E::store(dz + x, f * (s - p));
+    E::store(dz + x, f * (prob(E::load(z + x)) - p));
   }
 }
 
 // -------------------------------------------------------------------------------------------------------- planes
-// One lane per row; with C <= CM the classes stay in registers.
-template <typename T, int CM, int MODE>
+// VEC neighbouring rows per lane.  With C <= CM the classes stay in registers, else they are walked twice in blocks of 8; with
+// K <= KM so do the teacher's entries (their addresses differ from lane to lane: all are requested at once).
+template <typename T, int VEC>
+struct Px;
+template <>
+struct Px<float, 1> {
+  float r;
+  __device__ __forceinline__ void load(const float* p) { r = *p; }
+  __device__ __forceinline__ float get(int) const { return r; }
+  static __device__ __forceinline__ void store(float* p, const float* y) { *p = y[0]; }
+};
+template <>
+struct Px<bfu, 1> {
+  bfu r;
+  __device__ __forceinline__ void load(const bfu* p) { r = *p; }
+  __device__ __forceinline__ float get(int) const { return bf2f(r); }
+  static __device__ __forceinline__ void store(bfu* p, const float* y) { *p = f2bf(y[0]); }
+};
+template <>
+struct Px<bfu, 2> {
+  unsigned r;
+  __device__ __forceinline__ void load(const bfu* p) { r = *(const unsigned*)p; }
+  __device__ __forceinline__ float get(int i) const { return __builtin_bit_cast(float, i ? r & 0xffff0000u : r << 16); }
+  static __device__ __forceinline__ void store(bfu* p, const float* y) { *(unsigned*)p = (unsigned)f2bf(y[0]) | (unsigned)f2bf(y[1]) << 16; }
+};
+
+template <typename T, int VEC, int CM, int KM, int MODE>
 __global__ void __launch_bounds__(256) k_distill_planes(const DistP a) {
   using E = El<T>;
-  const long long row = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (row >= a.N) return;
-  const T* z = (const T*)a.z + row;
-  float x[CM > 0 ? CM : 1];
-  float m = -INFINITY, l = 0.f;
-  if (CM > 0) {
+  using P = Px<T, VEC>;
+  constexpr int BL = 8;
+  const long long first = ((long long)blockIdx.x * 256 + threadIdx.x) * VEC;
+  const bool in = first < a.N;
+  float total = 0.f;
+  if (in) {
+    const T* z = (const T*)a.z + first;
+    T* dz = (T*)a.dz + first;
+    P x[CM > 0 ? CM : BL];
+    float m[VEC], l[VEC];
 #pragma unroll
-    for (int c = 0; c < CM; ++c) x[c] = c < a.C ? E::load(z + c * a.z_cs) : -INFINITY;
-  }
-  if (MODE != BWD) {
-    if (CM > 0) {
+    for (int v = 0; v < VEC; ++v) m[v] = -INFINITY, l[v] = 0.f;
+    if constexpr (CM > 0) {
 #pragma unroll
-      for (int c = 0; c < CM; ++c) m = fmaxf(m, x[c]);
-      const float s = base_of(m);
+      for (int c = 0; c < CM; ++c)
+        if (c < a.C) x[c].load(z + c * a.z_cs);
+    }
+    // the teacher's entries of the lane's rows
+    int cl[KM > 0 ? KM * VEC : 1];
+    float tl[KM > 0 ? KM * VEC : 1], zl[KM > 0 ? KM * VEC : 1];
+    if constexpr (KM > 0) {
 #pragma unroll
-      for (int c = 0; c < CM; ++c) l += exp2_((x[c] - s) * a.c);
-    } else {
-      for (int c = 0; c < a.C; ++c) {
-        const float v = E::load(z + c * a.z_cs), M = fmaxf(m, v), s = base_of(M);
-        l = l * exp2_((m - s) * a.c) + exp2_((v - s) * a.c);
-        m = M;
+      for (int v = 0; v < VEC; ++v)
+#pragma unroll
+        for (int k = 0; k < KM; ++k)
+          if (k < a.K) cl[v * KM + k] = entry_class(a, first + v, k), tl[v * KM + k] = entry_logit(a, first + v, k);
+          else cl[v * KM + k] = -1;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v)
+#pragma unroll
+        for (int k = 0; k < KM; ++k) {
+          const int c = cl[v * KM + k];
+          zl[v * KM + k] = c >= 0 ? E::load(z + v + c * a.z_cs) : 0.f;
+        }
+    }
+    if (MODE != BWD) {
+      if constexpr (CM > 0) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+#pragma unroll
+          for (int c = 0; c < CM; ++c)
+            if (c < a.C) m[v] = fmaxf(m[v], x[c].get(v));
+          const float b = base_of(m[v]);
+#pragma unroll
+          for (int c = 0; c < CM; ++c)
+            if (c < a.C) l[v] += exp2_((x[c].get(v) - b) * a.c);
+        }
+      } else {
+        for (int c0 = 0; c0 < a.C; c0 += BL) {
+#pragma unroll
+          for (int c = 0; c < BL; ++c) x[c].load(z + min(c0 + c, a.C - 1) * a.z_cs);
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) {
+            float mx = m[v];
+#pragma unroll
+            for (int c = 0; c < BL; ++c) mx = fmaxf(mx, x[c].get(v));
+            const float b = base_of(mx);
+            l[v] *= exp2_((m[v] - b) * a.c);
+            m[v] = mx;
+#pragma unroll
+            for (int c = 0; c < BL; ++c) l[v] += c0 + c < a.C ? exp2_((x[c].get(v) - b) * a.c) : 0.f;
+          }
+        }
+      }
+    }
+    float l2[VEC], mt[VEC], lt2[VEC], f[VEC], fi[VEC];
+    bool empty[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      const long long row = first + v;
+      const auto entry = [&](int k) { return KM > 0 ? cl[v * KM + k] : entry_class(a, row, k); };
+      const auto logit = [&](int k) { return KM > 0 ? tl[v * KM + k] : entry_logit(a, row, k); };
+      mt[v] = -INFINITY;
+      float lt = 0.f;
+      if constexpr (KM > 0) {
+#pragma unroll
+        for (int k = 0; k < KM; ++k)
+          if (entry(k) >= 0) mt[v] = fmaxf(mt[v], logit(k));
+        const float b = base_of(mt[v]);
+#pragma unroll
+        for (int k = 0; k < KM; ++k)
+          if (entry(k) >= 0) lt += exp2_((logit(k) - b) * a.c);
+      } else {
+        for (int k = 0; k < a.K; ++k)
+          if (entry(k) >= 0) merge(mt[v], lt, logit(k), 1.f, a.c);
+      }
+      empty[v] = !(lt > 0.f) && lt == lt;
+      lt2[v] = log2_(lt);
+      if (MODE == BWD) m[v] = 0.f, l2[v] = a.lse_in[row] * LOG2E;
+      else l2[v] = log2_(l[v]);
+      if (MODE != BWD) {
+        float loss = 0.f;
+        const auto add = [&](int k) {
+          const int c = entry(k);
+          if (c < 0) return;
+          const float lp = (logit(k) - mt[v]) * a.c - lt2[v], p = exp2_(lp);
+          const float zc = KM > 0 ? zl[v * KM + k] : E::load(z + v + c * a.z_cs);
+          if (!(p == 0.f)) loss += p * (lp - ((zc - m[v]) * a.c - l2[v]));
+        };
+        if constexpr (KM > 0) {
+#pragma unroll
+          for (int k = 0; k < KM; ++k) add(k);
+        } else {
+          for (int k = 0; k < a.K; ++k) add(k);
+        }
+        loss = empty[v] ? 0.f : loss * LN2 * a.T * a.T * (a.w ? a.w[row] : 1.f);
+        if (a.loss_each) a.loss_rows[row] = loss;
+        total += loss;
+        if (MODE == FWD) a.lse[row] = (m[v] * a.c + l2[v]) * LN2;
+      }
+      if (MODE != FWD) f[v] = row_factor(a, row), fi[v] = MODE == BWD ? 0.f : f[v] * (1.f / l[v]);
+    }
+    if (MODE != FWD) {
+      const auto grad = [&](float x, int v) {
+        const float u = (x - m[v]) * a.c;
+        return MODE == BWD ? f[v] * exp2_(u - l2[v]) : fi[v] * exp2_(u);
+      };
+      if constexpr (CM > 0) {
+#pragma unroll
+        for (int c = 0; c < CM; ++c)
+          if (c < a.C) {
+            float y[VEC];
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) y[v] = empty[v] ? 0.f : grad(x[c].get(v), v);
+            P::store(dz + c * a.d_cs, y);
+          }
+      } else {
+        for (int c0 = 0; c0 < a.C; c0 += BL) {
+#pragma unroll
+          for (int c = 0; c < BL; ++c) x[c].load(z + min(c0 + c, a.C - 1) * a.z_cs);
+#pragma unroll
+          for (int c = 0; c < BL; ++c)
+            if (c0 + c < a.C) {
+              float y[VEC];
+#pragma unroll
+              for (int v = 0; v < VEC; ++v) y[v] = empty[v] ? 0.f : grad(x[c].get(v), v);
+              P::store(dz + (c0 + c) * a.d_cs, y);
+            }
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {  // the teacher's classes again, by the lane that wrote them; a class that stands there
+        if (empty[v]) continue;        // twice has both probabilities in its sum
+        const long long row = first + v;
+        if constexpr (KM > 0) {
+          float pk[KM];
+#pragma unroll
+          for (int k = 0; k < KM; ++k) pk[k] = cl[v * KM + k] >= 0 ? exp2_((tl[v * KM + k] - mt[v]) * a.c - lt2[v]) : 0.f;
+#pragma unroll
+          for (int k = 0; k < KM; ++k) {
+            const int c = cl[v * KM + k];
+            float p = 0.f;
+#pragma unroll
+            for (int j = 0; j < KM; ++j) p += cl[v * KM + j] == c ? pk[j] : 0.f;
+            if (c >= 0) E::store(dz + v + c * a.d_cs, grad(zl[v * KM + k], v) - f[v] * p);
+          }
+        } else {
+          for (int k = 0; k < a.K; ++k) {
+            const int c = entry_class(a, row, k);
+            if (c < 0) continue;
+            float p = 0.f;
+            for (int j = 0; j < a.K; ++j)
+              if (entry_class(a, row, j) == c) p += exp2_((entry_logit(a, row, j) - mt[v]) * a.c - lt2[v]);
+            E::store(dz + v + c * a.d_cs, grad(E::load(z + v + c * a.z_cs), v) - f[v] * p);
+          }
+        }
       }
     }
   }
-  float mt = -INFINITY, lt = 0.f;
-  for (int k = 0; k < a.K; ++k) {
-    const float t = entry_class(a, row, k) >= 0 ? entry_logit(a, row, k) : -INFINITY;
-    const float M = fmaxf(mt, t), s = base_of(M);
-    lt = lt * exp2_((mt - s) * a.c) + exp2_((t - s) * a.c);
-    mt = M;
-  }
-  const bool empty = !(lt > 0.f) && lt == lt;
-  const float lt2 = log2_(lt);
-  float l2;
-  if (MODE == BWD) m = 0.f, l2 = a.lse_in[row] * LOG2E;
-  else l2 = log2_(l);
-  if (MODE != BWD) {
-    float loss = 0.f;
-    for (int k = 0; k < a.K; ++k) {
-      const int cl = entry_class(a, row, k);
-      if (cl < 0) continue;
-      const float lp = (entry_logit(a, row, k) - mt) * a.c - lt2, p = exp2_(lp);
-      if (!(p == 0.f)) loss += p * (lp - ((E::load(z + cl * a.z_cs) - m) * a.c - l2));
-    }
-    a.loss_rows[row] = empty ? 0.f : loss * LN2 * a.T * a.T * (a.w ? a.w[row] : 1.f);
-    if (MODE == FWD) a.lse[row] = (m * a.c + l2) * LN2;
-  }
-  if (MODE == FWD) return;
-  const float f = row_factor(a, row), inv = MODE == BWD ? 0.f : 1.f / l;
-  const auto grad = [&](float v) {
-    const float u = (v - m) * a.c;
-    return MODE == BWD ? exp2_(u - l2) : exp2_(u) * inv;
-  };
-  T* dz = (T*)a.dz + row;
-  if (CM > 0) {
+  if (MODE != BWD && !a.loss_each) {  // one sum per workgroup
+    __shared__ float part[4];
 #pragma unroll
-    for (int c = 0; c < CM; ++c)
-      if (c < a.C) E::store(dz + c * a.d_cs, empty ? 0.f : f * grad(x[c]));
-  } else {
-    for (int c = 0; c < a.C; ++c) E::store(dz + c * a.d_cs, empty ? 0.f : f * grad(E::load(z + c * a.z_cs)));
-  }
-  if (empty) return;
-  for (int k = 0; k < a.K; ++k) {  // the teacher's classes again, by the lane that wrote them
-    const int cl = entry_class(a, row, k);
-    if (cl < 0) continue;
-    float p = 0.f;
-    for (int j = 0; j < a.K; ++j)
-      if (entry_class(a, row, j) == cl) p += exp2_((entry_logit(a, row, j) - mt) * a.c - lt2);
-    E::store(dz + cl * a.d_cs, f * (grad(E::load(z + cl * a.z_cs)) - p));
+    for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = total;
+    __syncthreads();
+    if (threadIdx.x == 0) a.loss_rows[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
   }
 }
 
-// Sum of the rows' losses by one workgroup, in 64 bits.
-__global__ void __launch_bounds__(1024) k_distill_sum(const float* __restrict__ rows, long long N, float scale, float* __restrict__ out) {
+// Sum of n losses (of rows, or of workgroups of planes) by one workgroup, in 64 bits; eight of a thread's loads in flight.
+__global__ void __launch_bounds__(1024) k_distill_sum(const float* __restrict__ x, long long n, float scale, float* __restrict__ out) {
   __shared__ double part[16];
   double s = 0.;
-  for (long long i = threadIdx.x; i < N; i += 1024) s += rows[i];
+  for (long long i = threadIdx.x; i < n; i += 8192) {
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = i + 1024 * j < n ? x[i + 1024 * j] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += (double)y[j];
+  }
 #pragma unroll
   for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
@@ -361,25 +496,34 @@ __global__ void __launch_bounds__(1024) k_distill_sum(const float* __restrict__ 
 // ----------------------------------------------------------------------------------------------------------- host
 template <typename T, int MODE>
 void launch_rows(const DistP& a, hipStream_t st) {
-  // Threads by the length of the row: a wave where that gives each lane at most 4 chunks, then workgroups of 256 and 1024.
-  const long long nch = ((long long)a.C + El<T>::EP - 1) / El<T>::EP + 1;
+  // Threads by the length of the row: a wave where that gives each lane at most 4 chunks, then workgroups whose registers hold
+  // the row while as many others as possible share the CU (their loads run under this one's arithmetic).
+  const int nch = a.C / El<T>::EP;  // whole chunks at most
   const dim3 grid((unsigned)a.N);
-#define GPN_ROWS(NT, CH) hipLaunchKernelGGL((k_distill_rows<T, NT, CH, MODE>), grid, dim3(NT), 0, st, a)
-  if (nch <= 64) GPN_ROWS(64, 1);
-  else if (nch <= 256) GPN_ROWS(64, 4);
-  else if (nch <= 1024) GPN_ROWS(256, 4);
-  else if (nch <= 2048) GPN_ROWS(256, 8);
-  else if (nch <= 4096) GPN_ROWS(1024, 4);
-  else if (nch <= 8192) GPN_ROWS(1024, 8);
-  else GPN_ROWS(1024, 16);
+#define GPN_ROWS(NT, CH, MANY) hipLaunchKernelGGL((k_distill_rows<T, NT, CH, MANY, MODE>), grid, dim3(NT), 0, st, a)
+  if (nch <= 64) GPN_ROWS(64, 1, false);
+  else if (nch <= 256) GPN_ROWS(64, 4, false);
+  else if (nch <= 1024) GPN_ROWS(256, 4, false);
+  else if (nch <= 2048) GPN_ROWS(256, 8, false);
+  else if (nch <= 4096) GPN_ROWS(512, 8, false);
+  else if (nch <= 8192) GPN_ROWS(512, 16, false);
+  else if (nch <= 16384) GPN_ROWS(1024, 16, false);
+  else GPN_ROWS(1024, 8, true);
 #undef GPN_ROWS
 }
 
-template <typename T, int MODE>
+template <typename T, int VEC, int MODE>
 void launch_planes(const DistP& a, hipStream_t st) {
-  const dim3 grid((unsigned)((a.N + 255) / 256));
-  if (a.C <= 32) hipLaunchKernelGGL((k_distill_planes<T, 32, MODE>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_distill_planes<T, 0, MODE>), grid, dim3(256), 0, st, a);
+  const dim3 grid((unsigned)((a.N + 256 * VEC - 1) / (256 * VEC)));
+#define GPN_PLANES(CM, KM) hipLaunchKernelGGL((k_distill_planes<T, VEC, CM, KM, MODE>), grid, dim3(256), 0, st, a)
+  if (a.C <= 32) {
+    if (a.K <= 8) GPN_PLANES(32, 8);
+    else GPN_PLANES(32, 0);
+  } else {
+    if (a.K <= 8) GPN_PLANES(0, 8);
+    else GPN_PLANES(0, 0);
+  }
+#undef GPN_PLANES
 }
 
 template <int MODE>
@@ -389,7 +533,7 @@ int run(const gpn_distill_args_t* x, hipStream_t st, const char* name) {
   GPN_REQUIRE(x->teacher_dtype == GPN_DT_F32 || x->teacher_dtype == GPN_DT_BF16, "%s: unknown teacher dtype %d", name, x->teacher_dtype);
   GPN_REQUIRE(x->index_bytes == 4 || x->index_bytes == 8, "%s: indices of %d bytes", name, x->index_bytes);
   GPN_REQUIRE(x->N >= 0 && x->N <= INT_MAX, "%s: %lld rows", name, x->N);
-  GPN_REQUIRE(x->C >= 1 && x->C <= (1 << 30), "%s: %d classes", name, x->C);
+  GPN_REQUIRE(x->C >= 1 && x->C <= (1 << 29), "%s: %d classes", name, x->C);
   GPN_REQUIRE(x->K >= 0 && x->K <= GPN_DISTILL_MAX_K, "%s: K must be in [0,%d] (got %d)", name, GPN_DISTILL_MAX_K, x->K);
   GPN_REQUIRE(x->temperature > 0.f && x->temperature < INFINITY, "%s: temperature must be positive and finite", name);
   GPN_REQUIRE(x->reduction >= GPN_RED_NONE && x->reduction <= GPN_RED_MEAN, "%s: unknown reduction %d", name, x->reduction);
@@ -419,13 +563,22 @@ int run(const gpn_distill_args_t* x, hipStream_t st, const char* name) {
   a.T = x->temperature, a.c = LOG2E / x->temperature;
   const float mean = x->reduction == GPN_RED_MEAN && x->N > 0 ? 1.f / (float)x->N : 1.f;
   a.grad_scale = mean * (MODE == STEP ? x->grad_scale : 1.f);
+  a.loss_each = x->reduction == GPN_RED_NONE;
+  long long losses = x->N;  // values in loss_rows that make up the loss
   if (x->N > 0) {
-    if (x->dtype == GPN_DT_F32) planes ? launch_planes<float, MODE>(a, st) : launch_rows<float, MODE>(a, st);
-    else planes ? launch_planes<bfu, MODE>(a, st) : launch_rows<bfu, MODE>(a, st);
+    // bf16 planes: two rows per lane where every plane starts on 4 bytes
+    const bool pairs = x->N % 2 == 0 && x->class_stride % 2 == 0 && x->dclass_stride % 2 == 0 &&
+                       (((size_t)x->logits | (size_t)x->dlogits) & 3) == 0;
+    if (planes) losses = (x->N + 255) / 256;
+    if (planes && x->dtype == GPN_DT_F32) launch_planes<float, 1, MODE>(a, st);
+    else if (planes && pairs) losses = (x->N + 511) / 512, launch_planes<bfu, 2, MODE>(a, st);
+    else if (planes) launch_planes<bfu, 1, MODE>(a, st);
+    else if (x->dtype == GPN_DT_F32) launch_rows<float, MODE>(a, st);
+    else launch_rows<bfu, MODE>(a, st);
     GPN_LAUNCH_CHECK(name);
   }
   if (MODE != BWD && x->reduction != GPN_RED_NONE) {
-    hipLaunchKernelGGL(k_distill_sum, dim3(1), dim3(1024), 0, st, x->loss_rows, x->N, mean, x->loss);
+    hipLaunchKernelGGL(k_distill_sum, dim3(1), dim3(1024), 0, st, x->loss_rows, losses, mean, x->loss);
     GPN_LAUNCH_CHECK("k_distill_sum");
   }
   return GPN_OK;
