@@ -28,6 +28,7 @@ typedef unsigned int u4v __attribute__((ext_vector_type(4)));
 
 namespace {
 
+constexpr int MAX_SPLIT = 64;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // ---------------------------------------------------------------------------------------------- matrix tiles per type
@@ -479,8 +480,8 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_fwd(const AttnP a) {
   store_cols<T, T, L::MD>(o, inv, (T*)a.out + (((long long)p.b * a.Lq + r.i) * a.Hq + r.hq) * a.D, a.D, h);
 }
 
-// Few rows (one tile of them, e.g. one new token of a sequence): the WK waves share the rows and divide the keys, each with
-// stages of its own and no barrier until their sums are joined.
+// Few rows (new tokens of sequences, or too few tiles to fill the card): the WK waves share a tile of rows and divide the keys,
+// each with stages of its own and no barrier until their sums are joined.
 template <typename T, int DP, int WK, int KT>
 struct Few {
   using L = Lay<T, DP>;
@@ -495,11 +496,12 @@ __global__ void __launch_bounds__(64 * WK, 2) k_attn_few(const AttnP a) {
   using M = Mt<T>;
   using L = Lay<T, DP>;
   constexpr int TM = M::TM, LO = F::LO;
-  int pr, split;
-  if (!locate(a.B * a.Hkv, a.nsplit, pr, split)) return;
+  int pr, unit;
+  if (!locate(a.B * a.Hkv, a.tiles * a.nsplit, pr, unit)) return;
+  const int split = unit / a.tiles, row0 = (a.tiles - 1 - (unit - split * a.tiles)) * TM;
   const Prob p = problem(a, pr);
   const int lane = threadIdx.x & 63, wave = wave_index(), n = lane & (TM - 1), h = lane / TM;
-  const Rows r = rows_of(a, p, 0, n, TM, split);
+  const Rows r = rows_of(a, p, row0, row0 + n, TM, split);
   if (a.D * (int)sizeof(T) < L::ROWB) clear_lds(attn_smem, (int)F::stage_bytes, F::NTH);
 
   const T* kb = (const T*)a.k + p.b * a.sk.b + p.hk * a.sk.h;
@@ -511,27 +513,36 @@ __global__ void __launch_bounds__(64 * WK, 2) k_attn_few(const AttnP a) {
     load_keys<T, DP, KT, 1>(kb, a.sk.l, a.D, j0, bits, base + buf * 2 * F::TILE, 0, lane);
     load_keys<T, DP, KT, 1>(vb, a.sv.l, a.D, j0, bits, base + (buf * 2 + 1) * F::TILE, 0, lane);
   };
+  // two stages on their way: the second lands while the first is worked on, whose memory the third then takes
+  constexpr int NEXT = WK * KT, LOADS = 2 * Dma<T, DP, KT, 1>::COUNT;
   const int jb = r.kbeg + wave * KT;
   keys.fetch(jb, lane);
-  unsigned long long bits = keys.bits(jb), next = 0;
+  unsigned long long bits = keys.bits(jb);
+  keys.fetch(jb + NEXT, lane);
   if (bits) request(jb, bits, 0);
-  keys.fetch(jb + WK * KT, lane);
+  unsigned long long next = keys.bits(jb + NEXT), after;
+  keys.fetch(jb + 2 * NEXT, lane);
+  if (next) request(jb + NEXT, next, 1);
   typename M::Frag qf[L::KF];
   load_frags<T, L::KF>(qf, r.live ? (const T*)a.q + p.b * a.sq.b + r.i * a.sq.l + r.hq * a.sq.h : nullptr, a.D, h);
   typename M::Acc o[L::MD];
 #pragma unroll
   for (int md = 0; md < L::MD; ++md) o[md] = (typename M::Acc)(0.f);
   float m = -INFINITY, l = 0.f;
-  stage_done<0, false>();
   int buf = 0;
-  for (int j0 = jb; j0 < r.kend; j0 += WK * KT, buf ^= 1, bits = next) {
-    next = keys.bits(j0 + WK * KT);
-    keys.fetch(j0 + 2 * WK * KT, lane);
-    if (next) request(j0 + WK * KT, next, buf ^ 1);
+  for (int j0 = jb; j0 < r.kend; j0 += NEXT, buf ^= 1, bits = next, next = after) {
+    if (next) stage_done<LOADS, false>();
+    else stage_done<0, false>();
     if (bits && !__all(r.lim < j0))
       attend<T, DP, KT>(mine + buf * 2 * F::TILE, mine + (buf * 2 + 1) * F::TILE, qf, o, m, l, bits, j0, r.lim, a.c, lane);
-    stage_done<0, false>();
+    after = keys.bits(j0 + 2 * NEXT);
+    keys.fetch(j0 + 3 * NEXT, lane);
+    if (after) {
+      stage_done<63, false>();  // the stage has been read (no wait for the loads)
+      request(j0 + 2 * NEXT, after, buf);
+    }
   }
+  stage_done<0, false>();
   l = col_sum<T>(l);
 
   float* mo = (float*)attn_smem;  // [WK][TM] references, [WK][TM] sums, [WK][TM][LO] outputs
@@ -550,19 +561,19 @@ __global__ void __launch_bounds__(64 * WK, 2) k_attn_few(const AttnP a) {
     }
   __syncthreads();
   for (int x = threadIdx.x; x < TM * (DP / 4); x += F::NTH) {
-    const int rw = x / (DP / 4), d = 4 * (x % (DP / 4));
+    const int rt = x / (DP / 4), rw = row0 + rt, d = 4 * (x % (DP / 4));
     if (rw >= a.M) continue;
     float mm = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < WK; ++w) mm = fmaxf(mm, mo[w * TM + rw]);
+    for (int w = 0; w < WK; ++w) mm = fmaxf(mm, mo[w * TM + rt]);
     const float ms = mm == -INFINITY ? 0.f : mm;
     float ll = 0.f;
     fl4 acc = (fl4)(0.f);
 #pragma unroll
     for (int w = 0; w < WK; ++w) {
-      const float f = exp2_((mo[w * TM + rw] - ms) * a.c);
-      ll += f * lo[w * TM + rw];
-      acc += f * *(const fl4*)(oo + (w * TM + rw) * LO + d);
+      const float f = exp2_((mo[w * TM + rt] - ms) * a.c);
+      ll += f * lo[w * TM + rt];
+      acc += f * *(const fl4*)(oo + (w * TM + rt) * LO + d);
     }
     acc *= ll > 0.f || ll != ll ? 1.f / ll : 0.f;
     const float l2 = ll == 0.f ? -INFINITY : ms * a.c + log2_(ll);
@@ -582,28 +593,37 @@ __global__ void __launch_bounds__(64 * WK, 2) k_attn_few(const AttnP a) {
   }
 }
 
-// Joins the splits of a row: every split left its own normalised output and log2-sum-exp.  32 lanes per row, 4 values a lane.
+// Joins the splits of a row: every split left its own normalised output and log2-sum-exp.  32 lanes per row, 4 values a lane;
+// lane s first looks at the splits s and s + 32.
 template <typename T>
 __global__ void __launch_bounds__(256) k_attn_join(const AttnP a) {
-  const long long x = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), rows = (long long)a.B * a.Hkv * a.M;
-  const int d = 4 * (threadIdx.x & 31);
+  static_assert(MAX_SPLIT <= 64, "two splits per lane");
+  const long long rows = (long long)a.B * a.Hkv * a.M, x = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int s0 = threadIdx.x & 31, d = 4 * s0;
+  const long long xr = x < rows ? x : rows - 1;
+  const float la = s0 < a.nsplit ? a.part_l[s0 * rows + xr] : -INFINITY;
+  const float lb = s0 + 32 < a.nsplit ? a.part_l[(s0 + 32) * rows + xr] : -INFINITY;
+  float mm = fmaxf(la, lb);
+  bool bad = la != la || lb != lb;
+#pragma unroll
+  for (int k = 16; k; k >>= 1) mm = fmaxf(mm, __shfl_xor(mm, k)), bad |= __shfl_xor((int)bad, k) != 0;
+  const float ms = mm == -INFINITY ? 0.f : mm;
+  const float wa = exp2_(la - ms), wb = exp2_(lb - ms);
+  float w = wa + wb;
+#pragma unroll
+  for (int k = 16; k; k >>= 1) w += __shfl_xor(w, k);
+  fl4 acc = (fl4)(0.f);
+  const float* o = a.part_o + xr * a.D + (d < a.D ? d : 0);
+  for (int s = 0; s < a.nsplit; s += 8) {  // eight parts on their way at once; those behind the last have no weight
+    fl4 y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] = *(const fl4*)(o + min(s + k, a.nsplit - 1) * rows * a.D);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc += (s + k < a.nsplit ? __shfl(s < 32 ? wa : wb, (s + k) & 31, 32) : 0.f) * y[k];
+  }
   if (x >= rows) return;
   const int pr = (int)(x / a.M), row = (int)(x - (long long)pr * a.M);
   const int b = pr / a.Hkv, i = row_pos(a, row), hq = (pr - b * a.Hkv) * a.G + row - i * a.G;
-  float mm = -INFINITY;
-  bool bad = false;
-  for (int s = 0; s < a.nsplit; ++s) {
-    const float l2 = a.part_l[s * rows + x];
-    mm = fmaxf(mm, l2), bad |= l2 != l2;
-  }
-  const float ms = mm == -INFINITY ? 0.f : mm;
-  float w = 0.f;
-  fl4 acc = (fl4)(0.f);
-  for (int s = 0; s < a.nsplit; ++s) {
-    const float f = exp2_(a.part_l[s * rows + x] - ms);
-    w += f;
-    if (d < a.D) acc += f * *(const fl4*)(a.part_o + (s * rows + x) * a.D + d);
-  }
   acc *= w > 0.f || bad ? 1.f / w : 0.f;
   if (d == 0) a.lse[((long long)b * a.Hq + hq) * a.Lq + i] = w == 0.f ? -INFINITY : (ms + log2_(w)) * LN2;
   typedef T V4 __attribute__((ext_vector_type(4)));
@@ -1094,29 +1114,25 @@ struct Plan {
   int bm, tiles, nsplit, split_keys;
 };
 
-constexpr int MAX_SPLIT = 64;
-
 Plan plan_forward(const gpn_attn_args_t* x) {
   Plan p;
   const bool f32 = x->dtype == GPN_DT_F32;
   const long long M = (long long)x->Lq * (x->Hq / x->Hkv), prob = (long long)x->B * x->Hkv;
-  p.few = M <= (f32 ? 16 : 32);
-  p.bm = p.few ? (f32 ? 16 : 32) : (f32 ? 64 : 128);
+  const int big = f32 ? 64 : 128, small = f32 ? 16 : 32;
+  // Tiles of few rows also where those of many would leave CUs idle and these do not (4 x 512 rows and keys, 8 heads of 64: 15
+  // against 21 us); wide fp32 heads apart, whose waves then find no room beside each other in LDS.
+  p.few = M <= small || (prob * ((M + big - 1) / big) < 256 && prob * ((M + small - 1) / small) >= 256 && !(f32 && x->D > 64));
+  p.bm = p.few ? small : big;
   p.tiles = (int)((M + p.bm - 1) / p.bm);
-  const int bn = p.few ? 128 : 64;
-  // Workgroups that find a CU of their own walk the keys alone; fewer than that, and the keys are cut, at 256 or more a
-  // part so that a part outweighs its share of the join.
-  const long long units = prob * p.tiles, want = 512;
+  // The card takes 512 workgroups (two per CU).  Where there are half as many or fewer the keys are cut too, into parts of
+  // min_part or more so that a part outweighs its share of the join.  (One query, 8 heads, 64 K keys: 64 parts 51 us, 5.3 TB/s;
+  // twice as many workgroups for eight queries of uneven lengths 82 against 76 us.)
+  const long long units = prob * p.tiles, min_part = f32 ? 128 : 256;
   p.nsplit = 1, p.split_keys = x->Lk;
-  if (units < want / 2 && x->Lk > 512) {
-    long long s = want / units;
-    if (s > MAX_SPLIT) s = MAX_SPLIT;
-    const long long most = x->Lk / 256;
-    if (s > most) s = most;
-    if (s > 1) {
-      p.split_keys = (int)(((x->Lk + s - 1) / s + bn - 1) / bn * bn);
-      p.nsplit = (x->Lk + p.split_keys - 1) / p.split_keys;
-    }
+  const long long s = units > 0 ? std::min({512 / units, x->Lk / min_part, (long long)MAX_SPLIT}) : 1;
+  if (s > 1) {
+    p.split_keys = (int)(((x->Lk + s - 1) / s + 63) / 64 * 64);
+    p.nsplit = (x->Lk + p.split_keys - 1) / p.split_keys;
   }
   return p;
 }
@@ -1169,9 +1185,9 @@ int forward_t(AttnP& a, const Plan& pl, hipStream_t st) {
   const long long grid = grid_of((long long)a.B * a.Hkv, (long long)pl.tiles * pl.nsplit);
   int rc;
   if (pl.few) {
-    constexpr int KT = F32 && DP > 64 ? 16 : 32;  // two stages of four waves' keys and values: at most 128 KB
-    using F = Few<T, DP, 4, KT>;
-    rc = launch(k_attn_few<T, DP, 4, KT>, "k_attn_few", grid, F::NTH, F::lds, st, a);
+    constexpr int KT = F32 && DP > 64 ? 16 : 32, WK = 16 * KT * Lay<T, DP>::ROWB > 64 * 1024 ? 2 : 4;  // two workgroups per CU
+    using F = Few<T, DP, WK, KT>;
+    rc = launch(k_attn_few<T, DP, WK, KT>, "k_attn_few", grid, F::NTH, F::lds, st, a);
   } else {
     constexpr int KT = F32 && DP > 64 ? 32 : 64;  // two stages of 64 KB at most: two workgroups per CU
     using F = Fwd<T, DP, 4, KT>;
