@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_dq(const AttnP a) {
   }
   float lse2 = r.live ? a.lse[at] * LOG2E : INFINITY;
   if (lse2 == -INFINITY) lse2 = INFINITY;  // a row without a key: every probability is zero
-  if (r.live && h == 0) a.delta[at] = delta, a.lse2[at] = lse2;
+  if (r.live && h == 0) a.delta[(long long)pr * a.M + r.row] = delta, a.lse2[(long long)pr * a.M + r.row] = lse2;
 
   typename M::Acc dq[L::MD];
 #pragma unroll
@@ -694,7 +694,6 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_dq(const AttnP a) {
     if (next) request(j0 + KT, next, buf ^ 1);
     if (bits && !__all(r.lim < j0)) {
       const bool partly = bits != Keys<KT>::ALL || __any(r.lim < j0 + KT - 1);
-      const unsigned long long lb = lane_bits<KT>(bits, j0, r.lim, h);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         const char* kt = attn_smem + buf * 2 * F::TILE + mt * TM * L::ROWB;
@@ -705,12 +704,14 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_dq(const AttnP a) {
           sc = M::mma(L::rowfrag(kt, f, lane), qf[f], sc);
           dp = M::mma(L::rowfrag(vt, f, lane), df[f], dp);
         }
+        if (partly) {  // a hidden score of -inf leaves a probability of zero
+          const unsigned long long lb = lane_bits<KT>(bits, j0, r.lim, h);
 #pragma unroll
-        for (int x = 0; x < M::NC; ++x) {
-          float e = exp2_(__builtin_fmaf(sc[x], a.c, -lse2));
-          if (partly && !(lb >> (mt * TM + M::crow(x, 0)) & 1)) e = 0.f;
-          sc[x] = e * (dp[x] - delta);
+          for (int x = 0; x < M::NC; ++x)
+            if (!(lb >> (mt * TM + M::crow(x, 0)) & 1)) sc[x] = -INFINITY;
         }
+#pragma unroll
+        for (int x = 0; x < M::NC; ++x) sc[x] = exp2_(__builtin_fmaf(sc[x], a.c, -lse2)) * (dp[x] - delta);
 #pragma unroll
         for (int t = 0; t < TM / 16; ++t) {
           const typename M::Frag sf = M::pack(sc, t);
@@ -767,23 +768,41 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) k_attn_dkv(const AttnP a) {
   const float* stats = (const float*)(attn_smem + F::stats_at);
   const char* vw = attn_smem + F::v_at + wn * TM * L::ROWB;
 
-  // Rows at and behind M are those of row M - 1 again, with a probability of zero.
+  // Where the group divides a round of loads (STEP rows), every lane's part of a row's address stays, and a stage is a uniform
+  // base on top; else row by row.  Rows at and behind M are those of row M - 1 again, with a probability of zero.
+  const bool even = Dm::NV == 1 && Dm::STEP % a.G == 0 && RB % a.G == 0 &&
+                    max(a.sq.l, a.sdo.l) < (1 << 20) && max(a.sq.h, a.sdo.h) < (1 << 20);
+  const int er = Dm::row(wave, lane, 0), ei = row_pos(a, er), eg = er - ei * a.G, ec = Dm::chunk(wave, lane, 0);
+  const unsigned eq = (unsigned)((ei * (int)a.sq.l + eg * (int)a.sq.h) * (int)sizeof(T) + ec * 16);
+  const unsigned ed = (unsigned)((ei * (int)a.sdo.l + eg * (int)a.sdo.h) * (int)sizeof(T) + ec * 16);
+  const bool mine = RB >= Dm::STEP || wave * Dm::RPI < RB, there = ec * M::EP < a.D;
+  const T* q0 = (const T*)a.q + p.b * a.sq.b + (long long)p.hk * a.G * a.sq.h;
+  const T* d0 = (const T*)a.dout + p.b * a.sdo.b + (long long)p.hk * a.G * a.sdo.h;
   const auto request = [&](int r0, int buf) {
-    const auto at = [&](const void* x, const Strides& s, int r) {
-      r = min(r0 + r, a.M - 1);
-      const int i = row_pos(a, r);
-      return (const T*)x + p.b * s.b + i * s.l + (p.hk * a.G + r - i * a.G) * s.h;
-    };
-    Dm::rows([&](int r) { return at(a.q, a.sq, r); }, a.D, base + buf * F::STAGE, wave, lane);
-    Dm::rows([&](int r) { return at(a.dout, a.sdo, r); }, a.D, base + buf * F::STAGE + F::TILE, wave, lane);
-    if (wave < 2) {
-      const int r = r0 + lane;
-      if (lane < RB) {
-        const int rr = min(r, a.M - 1), i = row_pos(a, rr);
-        const long long x = ((long long)p.b * a.Hq + p.hk * a.G + rr - i * a.G) * a.Lq + i;
-        const float* src = wave ? (r < a.M ? a.delta + x : (const float*)attn_zero) : (r < a.M ? a.lse2 + x : &attn_inf);
-        dma4(src, base + F::stats_at + buf * 512 + wave * 256);
+    const unsigned to = base + buf * F::STAGE;
+    if (even && r0 + RB <= a.M) {
+      const int i0 = row_pos(a, r0), is = Dm::STEP / a.G;
+      if (mine && there) {
+#pragma unroll
+        for (int i = 0; i < Dm::NI; ++i) {
+          dma16(q0 + (long long)(i0 + i * is) * a.sq.l, eq, to + (i * NW + wave) * 1024);
+          dma16(d0 + (long long)(i0 + i * is) * a.sdo.l, ed, to + F::TILE + (i * NW + wave) * 1024);
+        }
       }
+    } else {
+      const auto at = [&](const T* x, const Strides& s, int r) {
+        r = min(r0 + r, a.M - 1);
+        const int i = row_pos(a, r);
+        return x + i * s.l + (r - i * a.G) * s.h;
+      };
+      Dm::rows([&](int r) { return at(q0, a.sq, r); }, a.D, to, wave, lane);
+      Dm::rows([&](int r) { return at(d0, a.sdo, r); }, a.D, to + F::TILE, wave, lane);
+    }
+    if (wave < 2 && lane < RB) {
+      const int r = r0 + lane;
+      const float* src = wave ? (r < a.M ? a.delta + (long long)pr * a.M + r : (const float*)attn_zero)
+                              : (r < a.M ? a.lse2 + (long long)pr * a.M + r : &attn_inf);
+      dma4(src, base + F::stats_at + buf * 512 + wave * 256);
     }
   };
 
@@ -830,7 +849,6 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) k_attn_dkv(const AttnP a) {
       if (more) request(r0 + 2 * RB, buf == 0 ? 2 : buf - 1);
       const int rw = r0 + wr * F::RW;
       if (rw + F::RW > rany) {
-        const bool partly = rw < rall;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           const int lr = wr * F::RW + mt * TM;  // the tile's row in the stage
@@ -843,6 +861,12 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) k_attn_dkv(const AttnP a) {
             if constexpr (VL) dp = M::mma(L::rowfrag(dt, f, lane), L::rowfrag(vw, f, lane), dp);
             else dp = M::mma(L::rowfrag(dt, f, lane), vf[f], dp);
           }
+          if (rw < rall) {  // some rows do not see some keys: a score of -inf leaves a probability of zero
+            const int from = rmin - rw - mt * TM - 4 * h;
+#pragma unroll
+            for (int x = 0; x < M::NC; ++x)
+              if (M::crow(x, 0) < from) sc[x] = -INFINITY;
+          }
           const float* st = stats + buf * 128 + lr;
 #pragma unroll
           for (int q = 0; q < M::NC / 4; ++q) {
@@ -850,8 +874,7 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) k_attn_dkv(const AttnP a) {
             const fl4 l4 = *(const fl4*)(st + r), d4 = *(const fl4*)(st + 64 + r);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              float x = exp2_(__builtin_fmaf(sc[4 * q + e], a.c, -l4[e]));
-              if (partly && rw + mt * TM + r + e < rmin) x = 0.f;
+              const float x = exp2_(__builtin_fmaf(sc[4 * q + e], a.c, -l4[e]));
               sc[4 * q + e] = x;
               dp[4 * q + e] = x * (dp[4 * q + e] - d4[e]);
             }
@@ -1201,16 +1224,18 @@ int forward_t(AttnP& a, const Plan& pl, hipStream_t st) {
 // Keys of a workgroup of the dk / dv kernel: 4 waves' tiles.
 int dkv_keys(bool f32) { return f32 ? 64 : 128; }
 
-// Parts that the rows of a key tile are cut into: enough for two workgroups on every CU, with 256 rows or more each, so that a
-// part's products outweigh its sums' way through memory.
+// Parts that the rows of a key tile are cut into: one round of workgroups (one per CU; two for heads whose sums leave room), with
+// 256 rows or more each, so that a part's products outweigh its sums' way through memory.  (2 x 4096 causal, 4 key/value heads
+// of 128: 598 us with one round, 614 with two.)
 int plan_dkv(const gpn_attn_args_t* x) {
   const long long M = (long long)x->Lq * (x->Hq / x->Hkv);
   const int bn = dkv_keys(x->dtype == GPN_DT_F32);
   long long tiles = (x->Lk + bn - 1) / bn;
   if (x->causal) tiles = (tiles + 1) / 2;
   const long long units = (long long)x->B * x->Hkv * tiles;
-  if (units == 0 || units >= 256) return 1;
-  long long s = 512 / units;
+  const long long slots = x->D > 32 ? 256 : 512;
+  if (units == 0 || units > slots / 2) return 1;
+  long long s = slots / units;
   if (s > M / 256) s = M / 256;
   return s < 1 ? 1 : s > 16 ? 16 : (int)s;
 }
