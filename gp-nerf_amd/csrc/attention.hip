@@ -638,27 +638,28 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnP a) {
 // again from the row's log-sum-exp, so a row's share of the work needs no maximum and no sum:
 //   p = exp(s - lse), ds = p (do.v - delta), dq = scale sum ds k,  delta = do.o
 // delta and the log-sum-exp in powers of two (+inf for a row without a key) are left for the other kernel.
-template <typename T, int DP, int NW, int KT>
-__global__ void __launch_bounds__(64 * NW, 2) k_attn_dq(const AttnP a) {
+template <typename T, int DP, int NW, int KT, int WK>
+__global__ void __launch_bounds__(64 * NW * WK, 2) k_attn_dq(const AttnP a) {
   using F = Fwd<T, DP, NW, KT>;
   using M = Mt<T>;
   using L = Lay<T, DP>;
-  constexpr int TM = M::TM, MT = KT / TM;
+  constexpr int TM = M::TM, MT = KT / TM / WK, NTH = 64 * NW * WK;
+  static_assert(WK == 1 || WK == 2, "the join below is of two waves");
   int pr, unit;
   if (!locate(a.B * a.Hkv, a.tiles, pr, unit)) return;
   const int tile = a.tiles - 1 - unit;
   const Prob p = problem(a, pr);
-  const int lane = threadIdx.x & 63, wave = wave_index(), n = lane & (TM - 1), h = lane / TM;
-  const Rows r = rows_of(a, p, tile * F::BM, tile * F::BM + wave * TM + n, F::BM, 0);
-  if (a.D * (int)sizeof(T) < L::ROWB) clear_lds(attn_smem, (int)F::lds, F::NTH);
+  const int lane = threadIdx.x & 63, wave = wave_index(), wm = wave % NW, wk = wave / NW, n = lane & (TM - 1), h = lane / TM;
+  const Rows r = rows_of(a, p, tile * F::BM, tile * F::BM + wm * TM + n, F::BM, 0);
+  if (a.D * (int)sizeof(T) < L::ROWB) clear_lds(attn_smem, (int)F::lds, NTH);
 
   const T* kb = (const T*)a.k + p.b * a.sk.b + p.hk * a.sk.h;
   const T* vb = (const T*)a.v + p.b * a.sv.b + p.hk * a.sv.h;
   const unsigned base = lds_address(attn_smem);
   Keys<KT> keys = {a.key_mask ? a.key_mask + p.b * a.mask_sb : nullptr, r.kend, 0};
   const auto request = [&](int j0, unsigned long long bits, int buf) {
-    load_keys<T, DP, KT, NW>(kb, a.sk.l, a.D, j0, bits, base + buf * 2 * F::TILE, wave, lane);
-    load_keys<T, DP, KT, NW>(vb, a.sv.l, a.D, j0, bits, base + (buf * 2 + 1) * F::TILE, wave, lane);
+    load_keys<T, DP, KT, NW * WK>(kb, a.sk.l, a.D, j0, bits, base + buf * 2 * F::TILE, wave, lane);
+    load_keys<T, DP, KT, NW * WK>(vb, a.sv.l, a.D, j0, bits, base + (buf * 2 + 1) * F::TILE, wave, lane);
   };
   keys.fetch(0, lane);
   unsigned long long bits = keys.bits(0), next = 0;
@@ -681,7 +682,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_dq(const AttnP a) {
   }
   float lse2 = r.live ? a.lse[at] * LOG2E : INFINITY;
   if (lse2 == -INFINITY) lse2 = INFINITY;  // a row without a key: every probability is zero
-  if (r.live && h == 0) a.delta[(long long)pr * a.M + r.row] = delta, a.lse2[(long long)pr * a.M + r.row] = lse2;
+  if (r.live && h == 0 && wk == 0) a.delta[(long long)pr * a.M + r.row] = delta, a.lse2[(long long)pr * a.M + r.row] = lse2;
 
   typename M::Acc dq[L::MD];
 #pragma unroll
@@ -696,16 +697,18 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_dq(const AttnP a) {
       const bool partly = bits != Keys<KT>::ALL || __any(r.lim < j0 + KT - 1);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const char* kt = attn_smem + buf * 2 * F::TILE + mt * TM * L::ROWB;
+        const char* kt = attn_smem + buf * 2 * F::TILE + (wk * MT + mt) * TM * L::ROWB;
         const char* vt = kt + F::TILE;
         typename M::Acc sc = (typename M::Acc)(0.f), dp = (typename M::Acc)(0.f);
+        if (sizeof(T) == 2) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int f = 0; f < L::KF; ++f) {
           sc = M::mma(L::rowfrag(kt, f, lane), qf[f], sc);
           dp = M::mma(L::rowfrag(vt, f, lane), df[f], dp);
         }
+        __builtin_amdgcn_s_setprio(0);
         if (partly) {  // a hidden score of -inf leaves a probability of zero
-          const unsigned long long lb = lane_bits<KT>(bits, j0, r.lim, h);
+          const unsigned long long lb = lane_bits<KT>(bits, j0, r.lim, h) >> (wk * MT * TM);
 #pragma unroll
           for (int x = 0; x < M::NC; ++x)
             if (!(lb >> (mt * TM + M::crow(x, 0)) & 1)) sc[x] = -INFINITY;
@@ -721,6 +724,29 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_dq(const AttnP a) {
       }
     }
     stage_done<0, true>();
+  }
+  if constexpr (WK == 2) {  // the waves of the other half of every stage hand their sums over
+    fl4* x = (fl4*)attn_smem + wm * L::MD * (M::NC / 4) * 64 + lane;
+#pragma unroll
+    for (int md = 0; md < L::MD; ++md)
+#pragma unroll
+      for (int q = 0; q < M::NC / 4; ++q)
+        if (wk) {
+          fl4 y;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = dq[md][4 * q + e];
+          x[(md * (M::NC / 4) + q) * 64] = y;
+        }
+    __syncthreads();
+    if (wk) return;
+#pragma unroll
+    for (int md = 0; md < L::MD; ++md)
+#pragma unroll
+      for (int q = 0; q < M::NC / 4; ++q) {
+        const fl4 y = x[(md * (M::NC / 4) + q) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dq[md][4 * q + e] += y[e];
+      }
   }
   if (r.live) store_cols<T, T, L::MD>(dq, a.scale, (T*)a.dq + orow, a.D, h);
 }
@@ -855,12 +881,14 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) k_attn_dkv(const AttnP a) {
           const char* qt = attn_smem + buf * F::STAGE + lr * L::ROWB;
           const char* dt = qt + F::TILE;
           typename M::Acc sc = (typename M::Acc)(0.f), dp = (typename M::Acc)(0.f);
+          if (sizeof(T) == 2) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
           for (int f = 0; f < KF; ++f) {
             sc = M::mma(L::rowfrag(qt, f, lane), kf[f], sc);
             if constexpr (VL) dp = M::mma(L::rowfrag(dt, f, lane), L::rowfrag(vw, f, lane), dp);
             else dp = M::mma(L::rowfrag(dt, f, lane), vf[f], dp);
           }
+          __builtin_amdgcn_s_setprio(0);
           if (rw < rall) {  // some rows do not see some keys: a score of -inf leaves a probability of zero
             const int from = rmin - rw - mt * TM - 4 * h;
 #pragma unroll
@@ -1267,7 +1295,11 @@ int backward_t(AttnP& a, bool shrt, int nsplit, hipStream_t st) {
     constexpr int KT = F32 && DP > 64 ? 32 : 64;
     using F = Fwd<T, DP, 4, KT>;
     a.tiles = (a.M + F::BM - 1) / F::BM;
-    const int rc = launch(k_attn_dq<T, DP, 4, KT>, "k_attn_dq", grid_of(prob, a.tiles), F::NTH, F::lds, st, a);
+    // Where one workgroup per CU takes all tiles, eight waves share a tile's keys: two waves to a SIMD either way.
+    constexpr size_t join = (size_t)4 * F::L::MD * Mt<T>::NC * 64 * 4;
+    const int rc = prob * a.tiles > 256
+                       ? launch(k_attn_dq<T, DP, 4, KT, 1>, "k_attn_dq", grid_of(prob, a.tiles), 256, F::lds, st, a)
+                       : launch(k_attn_dq<T, DP, 4, KT, 2>, "k_attn_dq", grid_of(prob, a.tiles), 512, std::max(F::lds, join), st, a);
     if (rc) return rc;
   }
   using F = Dkv<T, DP, 4, 2>;
