@@ -480,6 +480,103 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_fwd(const AttnP a) {
   store_cols<T, T, L::MD>(o, inv, (T*)a.out + (((long long)p.b * a.Lq + r.i) * a.Hq + r.hq) * a.D, a.D, h);
 }
 
+// Up to KB keys (the samples of a ray): all of them are loaded at once and a row's softmax is taken in one piece.
+template <typename T, int DP, int NW, int KB>
+struct OnePiece {
+  using L = Lay<T, DP>;
+  static constexpr int TM = Mt<T>::TM, BM = NW * TM, NTH = 64 * NW, TILE = KB * L::ROWB;
+  static constexpr size_t lds = 2 * TILE;
+};
+
+template <typename T, int DP, int NW, int KB>
+__global__ void __launch_bounds__(64 * NW, 2) k_attn_one_piece(const AttnP a) {
+  using F = OnePiece<T, DP, NW, KB>;
+  using M = Mt<T>;
+  using L = Lay<T, DP>;
+  using Dm = Dma<T, DP, KB, NW>;
+  constexpr int TM = M::TM, MT = KB / TM, WORDS = KB / 64;
+  int pr, tile;
+  if (!locate(a.B * a.Hkv, a.tiles, pr, tile)) return;
+  const Prob p = problem(a, pr);
+  const int lane = threadIdx.x & 63, wave = wave_index(), n = lane & (TM - 1), h = lane / TM;
+  const Rows r = rows_of(a, p, tile * F::BM, tile * F::BM + wave * TM + n, F::BM, 0);
+  if (a.D * (int)sizeof(T) < L::ROWB) clear_lds(attn_smem, (int)F::lds, F::NTH);
+
+  const T* kb = (const T*)a.k + p.b * a.sk.b + p.hk * a.sk.h;
+  const T* vb = (const T*)a.v + p.b * a.sv.b + p.hk * a.sv.h;
+  const unsigned char* km = a.key_mask ? a.key_mask + p.b * a.mask_sb : nullptr;
+  const unsigned base = lds_address(attn_smem);
+  unsigned long long bits[WORDS];
+  bool all = true;
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) {
+    const int j = 64 * w + lane;
+    bits[w] = __ballot(j < r.kend && (!km || km[j]));
+    all &= bits[w] == ~0ull;
+  }
+  if (all && max(a.sk.l, a.sv.l) < (1 << 22)) {
+    Dm::whole(kb, a.sk.l, a.D, base, wave, lane);
+    Dm::whole(vb, a.sv.l, a.D, base + F::TILE, wave, lane);
+  } else {
+    const auto there = [&](int j) { return bits[WORDS == 1 ? 0 : j >> 6] >> (j & 63) & 1; };
+    Dm::rows([&](int j) { return there(j) ? kb + j * a.sk.l : (const T*)nullptr; }, a.D, base, wave, lane);
+    Dm::rows([&](int j) { return there(j) ? vb + j * a.sv.l : (const T*)nullptr; }, a.D, base + F::TILE, wave, lane);
+  }
+  typename M::Frag qf[L::KF];
+  load_frags<T, L::KF>(qf, r.live ? (const T*)a.q + p.b * a.sq.b + r.i * a.sq.l + r.hq * a.sq.h : nullptr, a.D, h);
+  stage_done<0, true>();
+
+  typename M::Acc sc[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    sc[mt] = (typename M::Acc)(0.f);
+#pragma unroll
+    for (int f = 0; f < L::KF; ++f) sc[mt] = M::mma(L::rowfrag(attn_smem + mt * TM * L::ROWB, f, lane), qf[f], sc[mt]);
+  }
+  if (!all || __any(r.lim < KB - 1)) {
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      const unsigned long long lb = lane_bits<64>(bits[w], 64 * w, r.lim, h);
+#pragma unroll
+      for (int mt = w * 64 / TM; mt < (w + 1) * 64 / TM; ++mt)
+#pragma unroll
+        for (int x = 0; x < M::NC; ++x)
+          if (!(lb >> (mt * TM - 64 * w + M::crow(x, 0)) & 1)) sc[mt][x] = -INFINITY;
+    }
+  }
+  float m = sc[0][0];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int x = 0; x < M::NC; ++x) m = fmaxf(m, sc[mt][x]);
+  m = col_max<T>(m);
+  const float mc = m == -INFINITY ? 0.f : m * a.c;
+  float l = 0.f;
+  typename M::Acc o[L::MD];
+#pragma unroll
+  for (int md = 0; md < L::MD; ++md) o[md] = (typename M::Acc)(0.f);
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+    for (int x = 0; x < M::NC; ++x) {
+      sc[mt][x] = exp2_(__builtin_fmaf(sc[mt][x], a.c, -mc));
+      l += sc[mt][x];
+    }
+#pragma unroll
+    for (int t = 0; t < TM / 16; ++t) {
+      const typename M::Frag pf = M::pack(sc[mt], t);
+#pragma unroll
+      for (int md = 0; md < L::MD; ++md)
+        o[md] = M::mma(L::colfrag(attn_smem + F::TILE + (mt * TM + 16 * t) * L::ROWB, md, lane), pf, o[md]);
+    }
+  }
+  l = col_sum<T>(l);
+  if (!r.live) return;
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // a row without a key is zero
+  if (h == 0) a.lse[((long long)p.b * a.Hq + r.hq) * a.Lq + r.i] = (l == 0.f ? -INFINITY : m * a.c + log2_(l)) * LN2;
+  store_cols<T, T, L::MD>(o, inv, (T*)a.out + (((long long)p.b * a.Lq + r.i) * a.Hq + r.hq) * a.D, a.D, h);
+}
+
 // Few rows (new tokens of sequences, or too few tiles to fill the card): the WK waves share a tile of rows and divide the keys,
 // each with stages of its own and no barrier until their sums are joined.
 template <typename T, int DP, int WK, int KT>
@@ -1161,6 +1258,7 @@ int launch(K kernel, const char* name, long long grid, int threads, size_t lds, 
 
 // How a forward call is cut: rows per workgroup, keys per stage, splits of the keys.
 struct Plan {
+  bool one_piece;  // few enough keys for one workgroup's registers
   bool few;  // one tile of rows per problem: the waves of a workgroup share the rows and divide the keys
   int bm, tiles, nsplit, split_keys;
 };
@@ -1172,6 +1270,13 @@ Plan plan_forward(const gpn_attn_args_t* x) {
   const int big = f32 ? 64 : 128, small = f32 ? 16 : 32;
   // Tiles of few rows also where those of many would leave CUs idle and these do not (4 x 512 rows and keys, 8 heads of 64: 15
   // against 21 us); wide fp32 heads apart, whose waves then find no room beside each other in LDS.
+  p.one_piece = x->Lk <= (f32 && x->D > 64 ? 64 : 128);  // 64 KB of keys and values: two workgroups per CU
+  if (p.one_piece) {  // as many waves as there are tiles of rows, four at most
+    p.few = false, p.nsplit = 1, p.split_keys = x->Lk;
+    p.bm = M <= small ? small : M <= 2 * small ? 2 * small : 4 * small;
+    p.tiles = (int)((M + p.bm - 1) / p.bm);
+    return p;
+  }
   p.few = M <= small || (prob * ((M + big - 1) / big) < 256 && prob * ((M + small - 1) / small) >= 256 && !(f32 && x->D > 64));
   p.bm = p.few ? small : big;
   p.tiles = (int)((M + p.bm - 1) / p.bm);
@@ -1235,6 +1340,14 @@ int forward_t(AttnP& a, const Plan& pl, hipStream_t st) {
   constexpr bool F32 = sizeof(T) == 4;
   const long long grid = grid_of((long long)a.B * a.Hkv, (long long)pl.tiles * pl.nsplit);
   int rc;
+  if (pl.one_piece) {
+    constexpr int TM = Mt<T>::TM;
+#define GPN_ONE(NW, KB) \
+  launch(k_attn_one_piece<T, DP, NW, KB>, "k_attn_one_piece", grid, 64 * NW, OnePiece<T, DP, NW, KB>::lds, st, a)
+    if (a.Lk <= 64) return pl.bm == TM ? GPN_ONE(1, 64) : pl.bm == 2 * TM ? GPN_ONE(2, 64) : GPN_ONE(4, 64);
+    if constexpr (!F32 || DP <= 64) return pl.bm == TM ? GPN_ONE(1, 128) : pl.bm == 2 * TM ? GPN_ONE(2, 128) : GPN_ONE(4, 128);
+#undef GPN_ONE
+  }
   if (pl.few) {
     constexpr int KT = F32 && DP > 64 ? 16 : 32, WK = 16 * KT * Lay<T, DP>::ROWB > 64 * 1024 ? 2 : 4;  // two workgroups per CU
     using F = Few<T, DP, WK, KT>;
