@@ -1084,15 +1084,17 @@ __global__ void __launch_bounds__(256) k_attn_dkv_join(const AttnP a) {
 
 // ------------------------------------------------------------------------------------- gradients of short sequences at once
 // Up to MB rows and MB keys (the samples of a ray): one workgroup holds the problem, reads it once and forms all five products;
-// the two kernels above would read it twice and take seven.  Every wave owns TM keys, walks all rows for its dk and dv, and
-// leaves ds in LDS by keys; then it owns TM rows and reads ds back by columns for dq.
+// the two kernels above would read it twice and take seven.  Every wave owns TM keys, walks the rows for its dk and dv, and
+// leaves ds in LDS by keys; then it owns TM rows and reads ds back by columns for dq.  128 rows go in two halves, so that ds
+// takes half the room and more workgroups share a CU; two waves then share a tile's dq, each with every other tile of keys.
 template <typename T, int DP, int MB>
 struct Short {
   using L = Lay<T, DP>;
-  using X = Lay<T, MB>;
+  static constexpr int HALVES = MB == 128 ? 2 : 1, HR = MB / HALVES;
+  using X = Lay<T, HR>;
   static constexpr int TM = Mt<T>::TM, NW = MB / TM, NTH = 64 * NW, TILE = MB * L::ROWB;
-  static constexpr int q_at = 0, do_at = TILE, k_at = 2 * TILE, x_at = 3 * TILE, st_at = x_at + MB * X::ROWB;
-  static constexpr size_t lds = st_at + 2 * MB * 4;
+  static constexpr int q_at = 0, do_at = TILE, k_at = 2 * TILE, x_at = 3 * TILE, st_at = x_at + MB * X::ROWB, dq_at = st_at + 2 * MB * 4;
+  static constexpr size_t lds = dq_at + (HALVES - 1) * NW / 2 * L::MD * Mt<T>::NC * 64 * 4;
   static constexpr bool fits = lds <= 128 * 1024;
 };
 
@@ -1166,8 +1168,9 @@ __global__ void __launch_bounds__(64 * MB / Mt<T>::TM, 2) k_attn_short(const Att
   typename M::Acc dk[MD], dv[MD];
 #pragma unroll
   for (int md = 0; md < MD; ++md) dk[md] = dv[md] = (typename M::Acc)(0.f);
-  // one tile of rows: its part of dv and dk, and ds -> LDS.  `partly`: some of the tile's rows do not see some of the keys.
-  const auto rows = [&](int r0, auto partly) {
+  // one tile of rows: its part of dv and dk, and ds -> LDS (columns from x0 on).  `partly`: some of the tile's rows do not see
+  // some of the keys.
+  const auto rows = [&](int r0, int x0, auto partly) {
     const char* qt = attn_smem + F::q_at + r0 * L::ROWB;
     const char* dt = attn_smem + F::do_at + r0 * L::ROWB;
     typename M::Acc sc = (typename M::Acc)(0.f), dp = (typename M::Acc)(0.f);
@@ -1202,44 +1205,79 @@ __global__ void __launch_bounds__(64 * MB / Mt<T>::TM, 2) k_attn_short(const Att
         V4 y;
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = sf[4 * g + e];
-        const int at = (r0 + M::crow(M::EP * t + 4 * g, h)) * (int)sizeof(T);
+        const int at = (r0 - x0 + M::crow(M::EP * t + 4 * g, h)) * (int)sizeof(T);
         *(V4*)(xs + xp * X::ROWB + ((at >> 4 ^ xw) << 4) + (at & 15)) = y;
       }
     }
   };
-  if (wave < ktiles) {
-    const bool hidden = __any(!seen);
-    int r0 = 0;
-    for (; r0 < a.M && r0 + TM <= rany; r0 += TM) {  // rows before the first that sees a key of the wave: ds is zero
+  const bool hidden = __any(!seen);
+  for (int half = 0; half < F::HALVES; ++half) {
+    const int x0 = half * F::HR, x1 = min(x0 + F::HR, a.M);
+    if (wave < ktiles) {
+      int r0 = x0;
+      for (; r0 < x1 && r0 + TM <= rany; r0 += TM) {  // rows before the first that sees a key of the wave: ds is zero
 #pragma unroll
-      for (int x = 0; x < TM * TM * (int)sizeof(T) / 1024; ++x) {
-        const int kx = wave * TM + lane % TM, at = r0 * (int)sizeof(T) + ((lane / TM) + x * (64 / TM)) * 16, px = X::phys(kx);
-        *(u4v*)(xs + px * X::ROWB + ((at >> 4 ^ X::swz(px)) << 4)) = u4v{0, 0, 0, 0};
+        for (int x = 0; x < TM * TM * (int)sizeof(T) / 1024; ++x) {
+          const int px = X::phys(wave * TM + lane % TM), at = (r0 - x0) * (int)sizeof(T) + ((lane / TM) + x * (64 / TM)) * 16;
+          *(u4v*)(xs + px * X::ROWB + ((at >> 4 ^ X::swz(px)) << 4)) = u4v{0, 0, 0, 0};
+        }
+      }
+      for (; r0 < x1 && (hidden || r0 < rall); r0 += TM) rows(r0, x0, std::true_type());
+      for (; r0 < x1; r0 += TM) rows(r0, x0, std::false_type());
+    }
+    if (half == F::HALVES - 1 && key < a.Lk) {
+      const long long at = (((long long)p.b * a.Lk + key) * a.Hkv + p.hk) * a.D;
+      store_cols<T, T, MD>(dk, a.scale, (T*)a.dk + at, a.D, h);
+      store_cols<T, T, MD>(dv, 1.f, (T*)a.dv + at, a.D, h);
+    }
+    __syncthreads();
+    constexpr int TW = NW / F::HALVES;  // tiles of rows of a half
+    const int tile = wave % TW, part = wave / TW, q0 = x0 + tile * TM;
+    typename M::Acc dq[MD];
+#pragma unroll
+    for (int md = 0; md < MD; ++md) dq[md] = (typename M::Acc)(0.f);
+    if (q0 < a.M) {
+      for (int kt = part; kt < ktiles; kt += F::HALVES) {
+#pragma unroll
+        for (int t = 0; t < TM / 16; ++t) {
+          const int j = kt * TM + 16 * t;
+          const typename M::Frag sf = X::colfrag(xs + j * X::ROWB, tile, lane);
+#pragma unroll
+          for (int md = 0; md < MD; ++md) dq[md] = M::mma(L::colfrag(attn_smem + F::k_at + j * L::ROWB, md, lane), sf, dq[md]);
+        }
       }
     }
-    for (; r0 < a.M && (hidden || r0 < rall); r0 += TM) rows(r0, std::true_type());
-    for (; r0 < a.M; r0 += TM) rows(r0, std::false_type());
-  }
-  if (key < a.Lk) {
-    const long long at = (((long long)p.b * a.Lk + key) * a.Hkv + p.hk) * a.D;
-    store_cols<T, T, MD>(dk, a.scale, (T*)a.dk + at, a.D, h);
-    store_cols<T, T, MD>(dv, 1.f, (T*)a.dv + at, a.D, h);
-  }
-  __syncthreads();
-  if (wave * TM >= a.M) return;
-  typename M::Acc dq[MD];
+    if constexpr (F::HALVES == 2) {
+      fl4* x = (fl4*)(attn_smem + F::dq_at) + tile * MD * (M::NC / 4) * 64 + lane;
+      if (part) {
 #pragma unroll
-  for (int md = 0; md < MD; ++md) dq[md] = (typename M::Acc)(0.f);
-  for (int kt = 0; kt < ktiles; ++kt) {
+        for (int md = 0; md < MD; ++md)
 #pragma unroll
-    for (int t = 0; t < TM / 16; ++t) {
-      const int j = kt * TM + 16 * t;
-      const typename M::Frag sf = X::colfrag(xs + j * X::ROWB, wave, lane);
+          for (int q = 0; q < M::NC / 4; ++q) {
+            fl4 y;
 #pragma unroll
-      for (int md = 0; md < MD; ++md) dq[md] = M::mma(L::colfrag(attn_smem + F::k_at + j * L::ROWB, md, lane), sf, dq[md]);
+            for (int e = 0; e < 4; ++e) y[e] = dq[md][4 * q + e];
+            x[(md * (M::NC / 4) + q) * 64] = y;
+          }
+      }
+      __syncthreads();
+      if (!part) {
+#pragma unroll
+        for (int md = 0; md < MD; ++md)
+#pragma unroll
+          for (int q = 0; q < M::NC / 4; ++q) {
+            const fl4 y = x[(md * (M::NC / 4) + q) * 64];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dq[md][4 * q + e] += y[e];
+          }
+      }
+    }
+    const int qr = q0 + n;
+    if (part == 0 && qr < a.M) {
+      const int qi = row_pos(a, qr), qh = p.hk * a.G + qr - qi * a.G;
+      store_cols<T, T, MD>(dq, a.scale, (T*)a.dq + (((long long)p.b * a.Lq + qi) * a.Hq + qh) * a.D, a.D, h);
     }
   }
-  if (live) store_cols<T, T, MD>(dq, a.scale, (T*)a.dq + orow, a.D, h);
 }
 
 // ------------------------------------------------------------------------------------------------------------ host
