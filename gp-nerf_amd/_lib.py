@@ -280,6 +280,13 @@ def dev_float(t, name, shape=None, dtype=None):
     return t
 
 
+def refuse_capture(name, instead):
+    """A graph that autograd records is not captured: a leaf that an eager graph holds too has its gradient summed on that graph's
+    stream, which a capture does not survive."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("%s: a graph that autograd records cannot be captured safely; capture %s instead" % (name, instead))
+
+
 def same_device(first, **others):
     for name, t in others.items():
         if t is not None and t.device != first.device:

@@ -140,9 +140,8 @@ def attention_backward(dout, q, k, v, out, lse, lengths=None, key_mask=None, cau
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, key_mask, causal, q_start, scale):
-        if any(ctx.needs_input_grad) and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("attention: a graph that autograd records cannot be captured safely (its leaves may belong to an "
-                               "eager graph on another stream); capture attention_forward and attention_backward instead")
+        if any(ctx.needs_input_grad):
+            _lib.refuse_capture("attention", "attention_forward and attention_backward")
         out, lse = attention_forward(q, k, v, lengths, key_mask, causal, q_start, scale)
         ctx.save_for_backward(q, k, v, out, lse, lengths, key_mask, q_start)
         ctx.causal, ctx.scale = causal, scale
@@ -151,6 +150,7 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        _lib.refuse_capture("attention", "attention_forward and attention_backward")
         q, k, v, out, lse, lengths, key_mask, q_start = ctx.saved_tensors
         grads = attention_backward(dout, q, k, v, out, lse, lengths, key_mask, ctx.causal, q_start, ctx.scale)
         return (*grads, None, None, None, None, None)

@@ -212,9 +212,17 @@ struct Dma {
   }
 };
 
-// Chunks at and beyond D are never loaded; a product's zero times whatever stands there has to be zero.
-__device__ __forceinline__ void clear_lds(char* lds, int bytes, int nth) {
-  for (int i = threadIdx.x * 16; i < bytes; i += nth * 16) *(u4v*)(lds + i) = u4v{0, 0, 0, 0};
+// A head narrower than DP: its last chunks are never loaded, and a product's zero times whatever stands there has to be zero.
+// `rows` rows of tiles that follow each other from lds on.
+template <typename T, int DP>
+__device__ __forceinline__ void clear_tail(char* lds, int rows, int D, int nth) {
+  using L = Lay<T, DP>;
+  const int c0 = D / Mt<T>::EP, nc = DP / Mt<T>::EP - c0;
+  if (nc <= 0) return;
+  for (int i = threadIdx.x; i < rows * nc; i += nth) {
+    const int r = i / nc, c = c0 + i - r * nc;
+    *(u4v*)(lds + r * L::ROWB + (c ^ L::swz(r)) * 16) = u4v{0, 0, 0, 0};
+  }
   __syncthreads();
 }
 
@@ -435,7 +443,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_fwd(const AttnP a) {
   const Prob p = problem(a, pr);
   const int lane = threadIdx.x & 63, wave = wave_index(), n = lane & (M::TM - 1), h = lane / M::TM;
   const Rows r = rows_of(a, p, tile * F::BM, tile * F::BM + wave * M::TM + n, F::BM, split);
-  if (a.D * (int)sizeof(T) < L::ROWB) clear_lds(attn_smem, (int)F::lds, F::NTH);
+  clear_tail<T, DP>(attn_smem, 4 * KT, a.D, F::NTH);
 
   const T* kb = (const T*)a.k + p.b * a.sk.b + p.hk * a.sk.h;
   const T* vb = (const T*)a.v + p.b * a.sv.b + p.hk * a.sv.h;
@@ -500,7 +508,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_one_piece(const AttnP a) {
   const Prob p = problem(a, pr);
   const int lane = threadIdx.x & 63, wave = wave_index(), n = lane & (TM - 1), h = lane / TM;
   const Rows r = rows_of(a, p, tile * F::BM, tile * F::BM + wave * TM + n, F::BM, 0);
-  if (a.D * (int)sizeof(T) < L::ROWB) clear_lds(attn_smem, (int)F::lds, F::NTH);
+  clear_tail<T, DP>(attn_smem, 2 * KB, a.D, F::NTH);
 
   const T* kb = (const T*)a.k + p.b * a.sk.b + p.hk * a.sk.h;
   const T* vb = (const T*)a.v + p.b * a.sv.b + p.hk * a.sv.h;
@@ -599,7 +607,7 @@ __global__ void __launch_bounds__(64 * WK, 2) k_attn_few(const AttnP a) {
   const Prob p = problem(a, pr);
   const int lane = threadIdx.x & 63, wave = wave_index(), n = lane & (TM - 1), h = lane / TM;
   const Rows r = rows_of(a, p, row0, row0 + n, TM, split);
-  if (a.D * (int)sizeof(T) < L::ROWB) clear_lds(attn_smem, (int)F::stage_bytes, F::NTH);
+  clear_tail<T, DP>(attn_smem, WK * 4 * KT, a.D, F::NTH);
 
   const T* kb = (const T*)a.k + p.b * a.sk.b + p.hk * a.sk.h;
   const T* vb = (const T*)a.v + p.b * a.sv.b + p.hk * a.sv.h;
@@ -748,7 +756,7 @@ __global__ void __launch_bounds__(64 * NW * WK, 2) k_attn_dq(const AttnP a) {
   const Prob p = problem(a, pr);
   const int lane = threadIdx.x & 63, wave = wave_index(), wm = wave % NW, wk = wave / NW, n = lane & (TM - 1), h = lane / TM;
   const Rows r = rows_of(a, p, tile * F::BM, tile * F::BM + wm * TM + n, F::BM, 0);
-  if (a.D * (int)sizeof(T) < L::ROWB) clear_lds(attn_smem, (int)F::lds, NTH);
+  clear_tail<T, DP>(attn_smem, 4 * KT, a.D, NTH);
 
   const T* kb = (const T*)a.k + p.b * a.sk.b + p.hk * a.sk.h;
   const T* vb = (const T*)a.v + p.b * a.sv.b + p.hk * a.sv.h;
@@ -933,7 +941,10 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) k_attn_dkv(const AttnP a) {
     const int tile = half ? a.tiles - 1 - tu : tu;
     if (half && tile <= tu) break;
     if (half) __syncthreads();  // the join of the first tile has been read
-    if ((half == 0 || WR > 1) && a.D * (int)sizeof(T) < L::ROWB) clear_lds(attn_smem, (int)F::stage_bytes, F::NTH);
+    if (half == 0 || WR > 1) {  // (the join has been here)
+      clear_tail<T, DP>(attn_smem, F::NBUF * 2 * RB, a.D, F::NTH);
+      if (VL) clear_tail<T, DP>(attn_smem + F::v_at, BN, a.D, F::NTH);
+    }
     const int j0 = tile * BN, key = j0 + wn * TM + n;
     const bool seen = key < p.len && (!km || km[key]);
     // first row that sees the lane's key / the wave's first key / all of the wave's keys
@@ -1109,7 +1120,7 @@ __global__ void __launch_bounds__(64 * MB / Mt<T>::TM, 2) k_attn_short(const Att
   if (!locate(a.B * a.Hkv, 1, pr, unit)) return;
   const Prob p = problem(a, pr);
   const int lane = threadIdx.x & 63, wave = wave_index(), n = lane & (TM - 1), h = lane / TM;
-  if (a.D * (int)sizeof(T) < L::ROWB) clear_lds(attn_smem, F::x_at, F::NTH);
+  clear_tail<T, DP>(attn_smem, 3 * MB, a.D, F::NTH);
   const unsigned base = lds_address(attn_smem);
   const unsigned char* km = a.key_mask ? a.key_mask + p.b * a.mask_sb : nullptr;
   const auto row_at = [&](const void* x, const Strides& s, int r) {
@@ -1283,7 +1294,7 @@ __global__ void __launch_bounds__(64 * MB / Mt<T>::TM, 2) k_attn_short(const Att
 // ------------------------------------------------------------------------------------------------------------ host
 template <typename K>
 int launch(K kernel, const char* name, long long grid, int threads, size_t lds, hipStream_t st, const AttnP& a) {
-  GPN_REQUIRE(grid <= INT_MAX, "%s: grid of %lld workgroups", name, grid);
+  GPN_REQUIRE(grid * threads < (1ll << 32), "%s: %lld workgroups of %d", name, grid, threads);
   if (grid == 0) return GPN_OK;
   if (lds > 64 * 1024) {
     hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);

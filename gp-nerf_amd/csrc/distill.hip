@@ -542,6 +542,7 @@ int run(const gpn_distill_args_t* x, hipStream_t st, const char* name) {
   const bool planes = x->class_stride != 1 && x->C > 1;
   GPN_REQUIRE(!planes || x->row_stride == 1 || x->N <= 1, "%s: logits need contiguous classes or contiguous rows (strides %lld, %lld)",
               name, x->row_stride, x->class_stride);
+  GPN_REQUIRE(planes || x->N <= GPN_DISTILL_MAX_ROWS, "%s: %lld rows of contiguous classes", name, x->N);
   if (MODE != BWD) {
     GPN_REQUIRE(x->loss_rows || x->N == 0, "%s: null loss_rows", name);
     GPN_REQUIRE(x->loss || x->reduction == GPN_RED_NONE, "%s: null loss", name);

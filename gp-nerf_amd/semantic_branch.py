@@ -156,9 +156,8 @@ def distill_topk_step(logits, teacher_logits, teacher_index, temperature=1.0, ro
 class _DistillTopK(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_logits, teacher_index, temperature, row_weight, reduction):
-        if ctx.needs_input_grad[0] and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("distill_topk_loss: a graph that autograd records cannot be captured safely (its leaves may belong "
-                               "to an eager graph on another stream); capture distill_topk_step instead")
+        if ctx.needs_input_grad[0]:
+            _lib.refuse_capture("distill_topk_loss", "distill_topk_step")
         loss, lse = distill_topk_forward(logits, teacher_logits, teacher_index, temperature, row_weight, reduction)
         ctx.save_for_backward(logits, teacher_logits, teacher_index, row_weight, lse)
         ctx.temperature, ctx.reduction = temperature, reduction
@@ -167,6 +166,7 @@ class _DistillTopK(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
+        _lib.refuse_capture("distill_topk_loss", "distill_topk_step")
         logits, t, x, w, lse = ctx.saved_tensors
         return (distill_topk_backward(dloss, logits, t, x, lse, ctx.temperature, w, ctx.reduction), None, None, None, None, None)
 

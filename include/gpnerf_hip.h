@@ -433,6 +433,7 @@ int gpn_attn_backward(const gpn_attn_args_t* a, gpn_stream_t stream);
  * gradient 0 whatever its logits hold.  The same class twice in a row counts twice.  The teacher takes no gradient.
  * dlogits may not overlap the logits.  N = 0 is a loss of 0. */
 #define GPN_DISTILL_MAX_K 256
+#define GPN_DISTILL_MAX_ROWS 4194303 /* where classes are contiguous: a workgroup of up to 1024 threads per row */
 #define GPN_RED_NONE 0
 #define GPN_RED_SUM 1
 #define GPN_RED_MEAN 2 /* over all N rows */
@@ -440,7 +441,7 @@ int gpn_attn_backward(const gpn_attn_args_t* a, gpn_stream_t stream);
 typedef struct {
   int dtype, teacher_dtype;   /* GPN_DT_* of logits and dlogits / of teacher */
   int index_bytes;            /* 4 or 8: index is int32 or int64 */
-  int C, K;
+  int C, K;                   /* classes (at most 2^29), teacher entries per row (at most GPN_DISTILL_MAX_K) */
   int reduction;              /* GPN_RED_* */
   float temperature;
   float grad_scale;           /* gpn_distill_step: dlogits is the gradient of grad_scale * loss */

@@ -450,3 +450,75 @@ def test_ray_attention_of_a_block():
         # chains of at most 64 + 16 + 48 + 64 (+ 432 rows for weights) sums of fp32: 700 half steps of 2^-24, times the
         # ratio of magnitudes summed to the largest result (below 2 here: random signs add up to less, not more)
         assert float((got.detach().cpu().double() - ref.detach()).abs().max()) <= 1400 * 2.0 ** -24 * max(1.0, float(ref.detach().abs().max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,shape,kw", [("bf16", (1, 300, 300, 4, 2, 128), dict(causal=True)), ("fp32", (2, 90, 200, 2, 2, 128), {}),
+                                            ("bf16", (40, 64, 64, 4, 4, 16), {}), ("fp32", (3, 128, 128, 2, 2, 32), {})], ids=str)
+def test_captured_kernels_of_every_path(dtype, shape, kw):
+    """The kernels with more LDS than a launch has by default, and those of short sequences, captured and replayed."""
+    x = _inputs(dtype, *shape)
+    cur = [t.clone() for t in x]
+    _both(*cur, **kw)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = _both(*cur, **kw)
+    for seed in (1, 2, 3):
+        new = _inputs(dtype, *shape, seed=seed)
+        for t, y in zip(cur, new):
+            t.copy_(y)
+        g.replay()
+        want = _both(*new, **kw)
+        torch.cuda.synchronize()
+        for n in want:
+            assert torch.equal(want[n], got[n]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("Lq,D", [(1, 128), (40, 64), (300, 64)])
+def test_offsets_past_32_bits(dtype, Lq, D):
+    """Keys, values and queries that lie more than 2^32 elements apart: between batches, and between positions."""
+    q, k, v, do = _inputs(dtype, 2, Lq, 20, 2, 1, D)
+    want = _both(q, k, v, do)
+    step = 2 ** 27 + 16
+    buf = torch.empty(20 * step + 2 * D + 64, dtype=q.dtype, device="cuda")  # about 5 (11) GB
+    far = lambda t, off, sb, sl, sh: buf.as_strided(t.shape, (sb, sl, sh, 1), off)  # noqa: E731
+    kk, vv = far(k, 0, D, step, 0), far(v, 64 + 2 * D, D, step, 0)  # positions apart
+    kk.copy_(k), vv.copy_(v)
+    got = _both(q, kk, vv, do)
+    for n in want:
+        assert torch.equal(want[n], got[n]), n
+    qq, dd = far(q, 0, 17 * step, 2 * D, D), far(do, 2 ** 21, 18 * step, 2 * D, D)  # batches apart
+    qq.copy_(q), dd.copy_(do)
+    got = _both(qq, k, v, dd)
+    for n in want:
+        assert torch.equal(want[n], got[n]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 64, 64, 1, 1, 16), (2, 40, 120, 3, 1, 16), (3, 128, 20, 2, 2, 32), (1, 20, 128, 4, 2, 64),
+                                   (2, 16, 100, 8, 1, 24), (4, 31, 33, 1, 1, 8)], ids=str)
+def test_short_sequences_with_masks(dtype, shape):
+    """Rows and keys that one workgroup holds: whole and partial tiles, masks, causal bounds that skip tiles."""
+    B, Lq, Lk = shape[:3]
+    x = _inputs(dtype, *shape)
+    g = torch.Generator().manual_seed(5)
+    mask = (torch.rand(B, Lk, generator=g) < 0.5).cuda()
+    lengths = torch.randint(0, Lk + 1, (B,), generator=g).to(torch.int32).cuda()
+    start = torch.randint(-Lq, Lk, (B,), generator=g).to(torch.int32).cuda()
+    _run(*x)
+    _run(*x, causal=True)
+    _run(*x, key_mask=mask, lengths=lengths)
+    _run(*x, key_mask=mask, lengths=lengths, causal=True, q_start=start)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("G", [1, 2, 3, 8, 24, 32])
+def test_groups_of_heads(dtype, G):
+    """Shared heads: groups that divide the tiles and those that do not, over several stages and parts."""
+    _run(*_inputs(dtype, 1, 150, 270, G, 1, 64), causal=True)
+    _run(*_inputs(dtype, 1, 37, 90, 2 * G, 2, 128))
