@@ -199,6 +199,17 @@ struct Dma {
       if (c * Mt<T>::EP < D) dma16(base + (long long)(i / NV * NV * STEP) * stride, off, lds + (i * NW + w) * 1024);
     }
   }
+  // uniform base + off(r) elements where there(r), else zero; 32-bit offsets
+  template <typename Off, typename There>
+  static __device__ __forceinline__ void near(const T* base, Off off, There there, int D, unsigned lds, int w, int lane) {
+    if (ROWS < STEP && w * RPI >= ROWS) return;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = chunk(w, lane, i), r = row(w, lane, i);
+      const char* p = (const char*)base + (unsigned)((off(r) + c * Mt<T>::EP) * (int)sizeof(T));
+      if (c * Mt<T>::EP < D) dma16(there(r) ? (const void*)p : (const void*)attn_zero, lds + (i * NW + w) * 1024);
+    }
+  }
   // rows by address: at(r) is the row, or null for one that reads as zero
   template <typename At>
   static __device__ __forceinline__ void rows(At at, int D, unsigned lds, int w, int lane) {
@@ -283,6 +294,18 @@ __device__ __forceinline__ void load_frags(typename Mt<T>::Frag (&f)[KF], const 
     const int d = 16 * i + Mt<T>::EP * h;
     u4v x = {0, 0, 0, 0};
     if (p && d < D) x = *(const u4v*)(p + d);
+    f[i] = __builtin_bit_cast(typename Mt<T>::Frag, x);
+  }
+}
+
+// the same at a wave-uniform base + the lane's 32-bit offset (elements)
+template <typename T, int KF>
+__device__ __forceinline__ void load_frags_near(typename Mt<T>::Frag (&f)[KF], const T* base, int off, bool there, int D, int h) {
+#pragma unroll
+  for (int i = 0; i < KF; ++i) {
+    const int d = 16 * i + Mt<T>::EP * h;
+    u4v x = {0, 0, 0, 0};
+    if (there && d < D) x = *(const u4v*)((const char*)base + (unsigned)((off + d) * (int)sizeof(T)));
     f[i] = __builtin_bit_cast(typename Mt<T>::Frag, x);
   }
 }
@@ -1123,49 +1146,62 @@ __global__ void __launch_bounds__(64 * MB / Mt<T>::TM, 2) k_attn_short(const Att
   clear_tail<T, DP>(attn_smem, 3 * MB, a.D, F::NTH);
   const unsigned base = lds_address(attn_smem);
   const unsigned char* km = a.key_mask ? a.key_mask + p.b * a.mask_sb : nullptr;
-  const auto row_at = [&](const void* x, const Strides& s, int r) {
+  // which keys are there; the first row and key of the problem, from which 32-bit offsets reach all others
+  constexpr int WORDS = (MB + 63) / 64;
+  unsigned long long bits[WORDS];
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) {
+    const int j = 64 * w + lane;
+    bits[w] = __ballot(j < p.len && (!km || km[j]));
+  }
+  const auto there = [&](int j) { return (bool)(bits[WORDS == 1 ? 0 : j >> 6] >> (j & 63) & 1); };
+  const T* q0 = (const T*)a.q + p.b * a.sq.b + (long long)p.hk * a.G * a.sq.h;
+  const T* d0 = (const T*)a.dout + p.b * a.sdo.b + (long long)p.hk * a.G * a.sdo.h;
+  const T* k0 = (const T*)a.k + p.b * a.sk.b + p.hk * a.sk.h;
+  const T* v0 = (const T*)a.v + p.b * a.sv.b + p.hk * a.sv.h;
+  const long long o0 = ((long long)p.b * a.Lq * a.Hq + p.hk * a.G) * a.D;  // of the problem's first row in out and dq
+  const auto off = [&](int r, int sl, int sh) {
     const int i = row_pos(a, r);
-    return (const T*)x + p.b * s.b + i * s.l + (p.hk * a.G + r - i * a.G) * s.h;
-  };
-  const auto key_at = [&](const void* x, const Strides& s, int j) {
-    return j < p.len && (!km || km[j]) ? (const T*)x + p.b * s.b + j * s.l + p.hk * s.h : (const T*)nullptr;
+    return i * sl + (r - i * a.G) * sh;
   };
   using Dm = Dma<T, DP, MB, NW>;
-  if (a.G == 1 && a.M == MB && max(a.sq.l, a.sdo.l) < (1 << 22)) {
-    Dm::whole(row_at(a.q, a.sq, 0), a.sq.l, a.D, base + F::q_at, wave, lane);
-    Dm::whole(row_at(a.dout, a.sdo, 0), a.sdo.l, a.D, base + F::do_at, wave, lane);
+  if (a.G == 1 && a.M == MB) {
+    Dm::whole(q0, a.sq.l, a.D, base + F::q_at, wave, lane);
+    Dm::whole(d0, a.sdo.l, a.D, base + F::do_at, wave, lane);
   } else {
-    Dm::rows([&](int r) { return r < a.M ? row_at(a.q, a.sq, r) : (const T*)nullptr; }, a.D, base + F::q_at, wave, lane);
-    Dm::rows([&](int r) { return r < a.M ? row_at(a.dout, a.sdo, r) : (const T*)nullptr; }, a.D, base + F::do_at, wave, lane);
+    const auto in = [&](int r) { return r < a.M; };
+    Dm::near(q0, [&](int r) { return off(min(r, a.M - 1), (int)a.sq.l, (int)a.sq.h); }, in, a.D, base + F::q_at, wave, lane);
+    Dm::near(d0, [&](int r) { return off(min(r, a.M - 1), (int)a.sdo.l, (int)a.sdo.h); }, in, a.D, base + F::do_at, wave, lane);
   }
-  if (!km && p.len == MB && a.sk.l < (1 << 22))
-    Dm::whole((const T*)a.k + p.b * a.sk.b + p.hk * a.sk.h, a.sk.l, a.D, base + F::k_at, wave, lane);
-  else
-    Dm::rows([&](int j) { return key_at(a.k, a.sk, j); }, a.D, base + F::k_at, wave, lane);
+  bool all = MB >= 64;
+#pragma unroll
+  for (int w = 0; w < WORDS; ++w) all &= bits[w] == ~0ull;
+  if (all) Dm::whole(k0, a.sk.l, a.D, base + F::k_at, wave, lane);
+  else Dm::near(k0, [&](int j) { return j * (int)a.sk.l; }, there, a.D, base + F::k_at, wave, lane);
 
   // the wave's keys
   const int key = wave * TM + n;
-  const bool seen = key_at(a.k, a.sk, key) != nullptr;
+  const bool seen = there(key);
   typename M::Frag kf[KF], vf[KF];
-  load_frags<T, KF>(kf, key_at(a.k, a.sk, key), a.D, h);
-  load_frags<T, KF>(vf, key_at(a.v, a.sv, key), a.D, h);
+  load_frags_near<T, KF>(kf, k0, key * (int)a.sk.l, seen, a.D, h);
+  load_frags_near<T, KF>(vf, v0, key * (int)a.sv.l, seen, a.D, h);
   // the wave's rows: log-sum-exp (powers of two; +inf: no probability) and do.o
   const int row = wave * TM + n;
   const bool live = row < a.M;
-  const int i = row_pos(a, live ? row : 0), hq = p.hk * a.G + (live ? row : 0) - i * a.G;
-  const long long orow = (((long long)p.b * a.Lq + i) * a.Hq + hq) * a.D;
   float* st = (float*)(attn_smem + F::st_at);  // [MB] log-sum-exp, [MB] delta
   {
+    const int rr = live ? row : 0, i = row_pos(a, rr);
     typename M::Frag of[KF], df[KF];
-    load_frags<T, KF>(of, live ? (const T*)a.out + orow : nullptr, a.D, h);
-    load_frags<T, KF>(df, live ? row_at(a.dout, a.sdo, row) : nullptr, a.D, h);
+    load_frags_near<T, KF>(of, (const T*)a.out + o0, off(rr, a.Hq * a.D, a.D), live, a.D, h);
+    load_frags_near<T, KF>(df, d0, off(rr, (int)a.sdo.l, (int)a.sdo.h), live, a.D, h);
     float delta = 0.f;
 #pragma unroll
     for (int f = 0; f < KF; ++f)
 #pragma unroll
       for (int e = 0; e < M::EP; ++e) delta = __builtin_fmaf((float)df[f][e], (float)of[f][e], delta);
     delta = col_sum<T>(delta);
-    float lse2 = live ? a.lse[((long long)p.b * a.Hq + hq) * a.Lq + i] * LOG2E : INFINITY;
+    const float* l0 = a.lse + ((long long)p.b * a.Hq + p.hk * a.G) * a.Lq;
+    float lse2 = live ? l0[(unsigned)((rr - i * a.G) * a.Lq + i)] * LOG2E : INFINITY;
     if (lse2 == -INFINITY) lse2 = INFINITY;
     if (h == 0) st[row] = lse2, st[MB + row] = delta;
   }
@@ -1237,9 +1273,10 @@ __global__ void __launch_bounds__(64 * MB / Mt<T>::TM, 2) k_attn_short(const Att
       for (; r0 < x1; r0 += TM) rows(r0, x0, std::false_type());
     }
     if (half == F::HALVES - 1 && key < a.Lk) {
-      const long long at = (((long long)p.b * a.Lk + key) * a.Hkv + p.hk) * a.D;
-      store_cols<T, T, MD>(dk, a.scale, (T*)a.dk + at, a.D, h);
-      store_cols<T, T, MD>(dv, 1.f, (T*)a.dv + at, a.D, h);
+      const long long g0 = ((long long)p.b * a.Lk * a.Hkv + p.hk) * a.D;
+      const unsigned at = (unsigned)(key * a.Hkv * a.D);
+      store_cols<T, T, MD>(dk, a.scale, (T*)a.dk + g0 + at, a.D, h);
+      store_cols<T, T, MD>(dv, 1.f, (T*)a.dv + g0 + at, a.D, h);
     }
     __syncthreads();
     constexpr int TW = NW / F::HALVES;  // tiles of rows of a half
@@ -1284,10 +1321,7 @@ __global__ void __launch_bounds__(64 * MB / Mt<T>::TM, 2) k_attn_short(const Att
       }
     }
     const int qr = q0 + n;
-    if (part == 0 && qr < a.M) {
-      const int qi = row_pos(a, qr), qh = p.hk * a.G + qr - qi * a.G;
-      store_cols<T, T, MD>(dq, a.scale, (T*)a.dq + (((long long)p.b * a.Lq + qi) * a.Hq + qh) * a.D, a.D, h);
-    }
+    if (part == 0 && qr < a.M) store_cols<T, T, MD>(dq, a.scale, (T*)a.dq + o0 + (unsigned)off(qr, a.Hq * a.D, a.D), a.D, h);
   }
 }
 
@@ -1437,10 +1471,18 @@ int short_t(const AttnP& a, hipStream_t st) {
   return gpn_set_error(GPN_E_ARG, "gpn_attn_backward: no such kernel");
 }
 
+// Strides that 128 rows times them, and their groups, stay far within 32 bits.
+bool is_near(const gpn_attn_args_t* x) {
+  const long long m = 1 << 20;
+  bool near = (long long)x->Hq * x->D < m;
+  for (int i = 1; i < 3; ++i) near &= x->q_stride[i] < m && x->k_stride[i] < m && x->v_stride[i] < m && x->dout_stride[i] < m;
+  return near;
+}
+
 // A problem that one workgroup's LDS holds with its ds: 128 rows and keys, at most this wide.
 bool is_short(const gpn_attn_args_t* x) {
   const long long n = std::max((long long)x->Lq * (x->Hq / x->Hkv), (long long)x->Lk);
-  return n >= 1 && n <= 128 && x->D <= (x->dtype == GPN_DT_BF16 || n <= 64 ? 64 : 32);
+  return n >= 1 && n <= 128 && x->D <= (x->dtype == GPN_DT_BF16 || n <= 64 ? 64 : 32) && is_near(x);
 }
 
 template <typename T, int DP>
