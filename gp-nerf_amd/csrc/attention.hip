@@ -298,7 +298,15 @@ __device__ __forceinline__ void load_frags(typename Mt<T>::Frag (&f)[KF], const 
   }
 }
 
-// the same at a wave-uniform base + the lane's 32-bit offset (elements)
+// A use of loaded values before a loop of asynchronous loads: the compiler, which knows nothing of those, would else wait for
+// its own loads at their first use inside the loop, in every turn, and with them for the stage just requested.
+template <typename F, int N>
+__device__ __forceinline__ void settle(F (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
+
+// load_frags at a wave-uniform base + the lane's 32-bit offset (elements)
 template <typename T, int KF>
 __device__ __forceinline__ void load_frags_near(typename Mt<T>::Frag (&f)[KF], const T* base, int off, bool there, int D, int h) {
 #pragma unroll
@@ -487,6 +495,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_fwd(const AttnP a) {
 #pragma unroll
   for (int md = 0; md < L::MD; ++md) o[md] = (typename M::Acc)(0.f);
   float m = -INFINITY, l = 0.f;  // reference of the raw scores; this lane's share of the sum
+  settle(qf);
   stage_done<0, true>();
   int buf = 0;
   for (int j0 = r.kbeg; j0 < r.kend; j0 += KT, buf ^= 1, bits = next) {
@@ -657,6 +666,7 @@ __global__ void __launch_bounds__(64 * WK, 2) k_attn_few(const AttnP a) {
 #pragma unroll
   for (int md = 0; md < L::MD; ++md) o[md] = (typename M::Acc)(0.f);
   float m = -INFINITY, l = 0.f;
+  settle(qf);
   int buf = 0;
   for (int j0 = jb; j0 < r.kend; j0 += NEXT, buf ^= 1, bits = next, next = after) {
     if (next) stage_done<LOADS, false>();
@@ -815,6 +825,8 @@ __global__ void __launch_bounds__(64 * NW * WK, 2) k_attn_dq(const AttnP a) {
   typename M::Acc dq[L::MD];
 #pragma unroll
   for (int md = 0; md < L::MD; ++md) dq[md] = (typename M::Acc)(0.f);
+  settle(qf), settle(df);
+  asm volatile("" : "+v"(lse2), "+v"(delta));
   stage_done<0, true>();
   int buf = 0;
   for (int j0 = 0; j0 < r.kend; j0 += KT, buf ^= 1, bits = next) {
@@ -999,6 +1011,8 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) k_attn_dkv(const AttnP a) {
     for (int md = 0; md < MD; ++md) dk[md] = dv[md] = (typename M::Acc)(0.f);
     if (rbeg < rend) request(rbeg, 0);
     if (rbeg + RB < rend) request(rbeg + RB, 1);
+    settle(kf);
+    if (!VL) settle(vf);
     stage_done<0, true>();
     int buf = 0;
     for (int r0 = rbeg; r0 < rend; r0 += RB) {
