@@ -903,7 +903,7 @@ struct Dkv {
   using M = Mt<T>;
   using L = Lay<T, DP>;
   static constexpr int TM = M::TM, RW = sizeof(T) == 4 && DP > 64 ? 16 : 32, RB = WR * RW, MT = RW / TM, BN = WN * TM;
-  static constexpr int NW = WN * WR, NTH = 64 * NW, TILE = RB * L::ROWB, STAGE = 2 * TILE, NBUF = 3;
+  static constexpr int NW = WN * WR, NTH = 64 * NW, TILE = RB * L::ROWB, STAGE = 2 * TILE, NBUF = WR == 1 && DP > 64 ? 2 : 3;
   static constexpr bool VL = DP > 64;
   static constexpr int stats_at = NBUF * STAGE, v_at = stats_at + NBUF * 512;  // [NBUF][2][64] floats; values
   static constexpr size_t stage_bytes = v_at + (VL ? BN * L::ROWB : 0);
@@ -1010,14 +1010,14 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) k_attn_dkv(const AttnP a) {
 #pragma unroll
     for (int md = 0; md < MD; ++md) dk[md] = dv[md] = (typename M::Acc)(0.f);
     if (rbeg < rend) request(rbeg, 0);
-    if (rbeg + RB < rend) request(rbeg + RB, 1);
+    if (F::NBUF == 3 && rbeg + RB < rend) request(rbeg + RB, 1);
     settle(kf);
     if (!VL) settle(vf);
     stage_done<0, true>();
     int buf = 0;
     for (int r0 = rbeg; r0 < rend; r0 += RB) {
-      const bool more = r0 + 2 * RB < rend;
-      if (more) request(r0 + 2 * RB, buf == 0 ? 2 : buf - 1);
+      const bool more = r0 + (F::NBUF - 1) * RB < rend;
+      if (more) request(r0 + (F::NBUF - 1) * RB, F::NBUF == 2 ? buf ^ 1 : buf == 0 ? 2 : buf - 1);
       const int rw = r0 + wr * F::RW;
       if (rw + F::RW > rany) {
 #pragma unroll
@@ -1064,9 +1064,9 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) k_attn_dkv(const AttnP a) {
         }
       }
       // the next stage has landed; the one after it may be on its way
-      if (more) stage_done<F::LOADS, true>();
+      if (F::NBUF == 3 && more) stage_done<F::LOADS, true>();
       else stage_done<0, true>();
-      buf = buf == 2 ? 0 : buf + 1;
+      buf = buf == F::NBUF - 1 ? 0 : buf + 1;
     }
     if constexpr (WR == 2) {  // wave 0 of a pair finishes dk, wave 1 finishes dv
       fl4* x = (fl4*)attn_smem + (wn * 2) * MD * (M::NC / 4) * 64 + lane;
@@ -1499,6 +1499,13 @@ bool is_short(const gpn_attn_args_t* x) {
   return n >= 1 && n <= 128 && x->D <= (x->dtype == GPN_DT_BF16 || n <= 64 ? 64 : 32) && is_near(x);
 }
 
+template <typename T, int DP, int WR>
+int dkv_t(const AttnP& a, long long grid, hipStream_t st) {
+  using F = Dkv<T, DP, 4, WR>;
+  static_assert(F::BN == (sizeof(T) == 4 ? 64 : 128) && F::lds <= 160 * 1024, "dkv_keys, LDS");
+  return launch(k_attn_dkv<T, DP, 4, WR>, "k_attn_dkv", grid, F::NTH, F::lds, st, a);
+}
+
 template <typename T, int DP>
 int backward_t(AttnP& a, bool shrt, int nsplit, hipStream_t st) {
   constexpr bool F32 = sizeof(T) == 4;
@@ -1520,11 +1527,13 @@ int backward_t(AttnP& a, bool shrt, int nsplit, hipStream_t st) {
                        : launch(k_attn_dq<T, DP, 4, KT, 2>, "k_attn_dq", grid_of(prob, a.tiles), 512, std::max(F::lds, join), st, a);
     if (rc) return rc;
   }
-  using F = Dkv<T, DP, 4, 2>;
-  static_assert(F::BN == (F32 ? 64 : 128) && F::lds <= 160 * 1024, "dkv_keys, LDS");
-  a.tiles = (a.Lk + F::BN - 1) / F::BN, a.nsplit = nsplit;
-  const long long units = (long long)(a.causal ? (a.tiles + 1) / 2 : a.tiles) * nsplit;
-  const int rc = launch(k_attn_dkv<T, DP, 4, 2>, "k_attn_dkv", grid_of(prob, units), F::NTH, F::lds, st, a);
+  a.tiles = (a.Lk + dkv_keys(F32) - 1) / dkv_keys(F32), a.nsplit = nsplit;
+  const long long units = (long long)(a.causal ? (a.tiles + 1) / 2 : a.tiles) * nsplit, grid = grid_of(prob, units);
+  // Pairs of waves per key tile keep the parts few where there are few tiles; with two workgroups for every CU in any case,
+  // workgroups of four waves wait for each other less (4 x 4096 of 16 heads of 64: 1107 us for the backward in pairs, 1062).
+  int rc;
+  if (!F32 && prob * units >= 512) rc = dkv_t<T, DP, F32 ? 2 : 1>(a, grid, st);
+  else rc = dkv_t<T, DP, 2>(a, grid, st);
   if (rc || nsplit == 1) return rc;
   return launch(k_attn_dkv_join<T>, "k_attn_dkv_join", ((long long)a.B * a.Lk * a.Hkv * a.D / 2 + 255) / 256, 256, 0, st, a);
 }

@@ -519,3 +519,12 @@ def test_groups_of_heads(dtype, G):
     """Shared heads: groups that divide the tiles and those that do not, over several stages and parts."""
     _run(*_inputs(dtype, 1, 150, 270, G, 1, 64), causal=True)
     _run(*_inputs(dtype, 1, 37, 90, 2 * G, 2, 128))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape,causal", [((130, 140, 150, 4, 4, 128), False), ((130, 150, 150, 4, 4, 72), True),
+                                          ((65, 150, 300, 8, 8, 24), True)], ids=str)
+def test_many_problems(dtype, shape, causal):
+    """More problems than workgroups fit the card at once."""
+    _run(*_inputs(dtype, *shape), causal=causal)
