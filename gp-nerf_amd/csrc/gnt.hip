@@ -1327,7 +1327,7 @@ k_view_attn(gpn_view_layer_t Lw, const float* q_in, const float* __restrict__ fe
     return or_over_g(o ? 1u : 0u) != 0;
   };
   f2 l2e = (f2){LOG2E_F, LOG2E_F};
-  asm volatile("" : "+v"(l2e));  // keep log2(e) in registers: a literal operand blocks v_pk_fma_f32
+  asm volatile("" : "+v"(l2e));  // keep log2(e) in a register, not a literal in every fma
   VA_T0();
   for (;;) {
     VA_MARK(5);
@@ -2456,7 +2456,7 @@ __device__ __forceinline__ unsigned rl_u(unsigned v, int l) {
 template <int DEPTH>
 __global__ void __launch_bounds__(SEM_RAYS * 64, SEM_WAVES_PER_SIMD)
 k_sem(gpn_sem_args_t a, int strip_groups) {
-  constexpr int LP = (DEPTH + 1) / 2;  // layers are processed in pairs (v_pk_fma_f32)
+  constexpr int LP = (DEPTH + 1) / 2;  // layers are processed in pairs
   __shared__ float sP[GPN_MAX_VIEWS * 12];
   __shared__ __attribute__((aligned(16))) float sH[SEM_RAYS][LP * 16];
   __shared__ __attribute__((aligned(16))) float sW[LP * 4 * 64 * 4];
@@ -2520,7 +2520,7 @@ k_sem(gpn_sem_args_t a, int strip_groups) {
   const bool dense = a.deep_dense != nullptr;
   // attn_fc[2] of every layer: this lane's row (its channel group) of the [64,8] weight and its
   // bias, scaled by log2(e) so that the softmax weight is a bare v_exp_f32; layers l = 2p, 2p+1
-  // sit in the two halves of an f2 (one v_pk_fma_f32 per hidden value and layer pair)
+  // sit in the two halves of an f2 (two fma per hidden value and layer pair)
   // (weights live in LDS, one 16-byte unit per lane, layer pair and pair of hidden values:
   // (w[2p][k], w[2p+1][k], w[2p][k+1], w[2p+1][k+1]); 72 registers fewer = twice the waves per SIMD)
   f2 a2b[LP];
@@ -2671,7 +2671,7 @@ k_sem(gpn_sem_args_t a, int strip_groups) {
       float w3 = w3u, w2 = w2u;
       if (vis != 0) {
         // logits of this lane's channel group in all layers: attn_fc[2] row . hidden + bias (:66-70),
-        // two layers per packed fma; softmax weight = 2^(logit - lse) in log2 units
+        // two layers at a time; softmax weight = 2^(logit - lse) in log2 units
         const float* hp = sH[wave];
         f2 w3p = (f2){0.f, 0.f}, w2p = (f2){0.f, 0.f};
 #pragma unroll
