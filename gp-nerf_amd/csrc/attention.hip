@@ -1365,8 +1365,6 @@ Plan plan_forward(const gpn_attn_args_t* x) {
   const bool f32 = x->dtype == GPN_DT_F32;
   const long long M = (long long)x->Lq * (x->Hq / x->Hkv), prob = (long long)x->B * x->Hkv;
   const int big = f32 ? 64 : 128, small = f32 ? 16 : 32;
-  // Tiles of few rows also where those of many would leave CUs idle and these do not (4 x 512 rows and keys, 8 heads of 64: 15
-  // against 21 us); wide fp32 heads apart, whose waves then find no room beside each other in LDS.
   p.one_piece = x->Lk <= (f32 && x->D > 64 ? 64 : 128);  // 64 KB of keys and values: two workgroups per CU
   if (p.one_piece) {  // as many waves as there are tiles of rows, four at most
     p.few = false, p.nsplit = 1, p.split_keys = x->Lk;
@@ -1374,15 +1372,22 @@ Plan plan_forward(const gpn_attn_args_t* x) {
     p.tiles = (int)((M + p.bm - 1) / p.bm);
     return p;
   }
-  p.few = M <= small || (prob * ((M + big - 1) / big) < 256 && prob * ((M + small - 1) / small) >= 256 && !(f32 && x->D > 64));
+  // Tiles of few rows also where those of many would leave half the CUs or more without work and these do not (4 x 512 rows
+  // and keys, 8 heads of 64: 15 against 21 us).  Nearer a full card the four times as many reads of the keys cost more (3 x 777,
+  // 8 query and 2 key/value heads of 128: 43 against 28 us).  Wide fp32 heads apart, whose waves then find no room beside each
+  // other in LDS.
+  p.few = M <= small || (prob * ((M + big - 1) / big) <= 128 && prob * ((M + small - 1) / small) >= 256 && !(f32 && x->D > 64));
   p.bm = p.few ? small : big;
   p.tiles = (int)((M + p.bm - 1) / p.bm);
-  // The card takes 512 workgroups (two per CU).  Where there are half as many or fewer the keys are cut too, into parts of
-  // min_part or more so that a part outweighs its share of the join.  (One query, 8 heads, 64 K keys: 64 parts 51 us, 5.3 TB/s;
-  // twice as many workgroups for eight queries of uneven lengths 82 against 76 us.)
+  // The card takes 512 workgroups (two per CU).  Few rows that leave half the room or more have their keys cut too, into parts
+  // of min_part or more so that a part outweighs its share of the join (one query, 8 heads, 64 K keys: 64 parts 51 us, 5.3 TB/s;
+  // twice as many workgroups for eight queries of uneven lengths 82 against 76 us).  So do tiles of many rows that leave half
+  // the CUs without work; with more, what the join reads and writes costs what the parts gain (5 x 777, 8 query and 2 key/value
+  // heads of 64, 250 workgroups: 33 us in two parts, 23 in one).
   const long long units = prob * p.tiles, min_part = f32 ? 128 : 256;
   p.nsplit = 1, p.split_keys = x->Lk;
-  const long long s = units > 0 ? std::min({512 / units, x->Lk / min_part, (long long)MAX_SPLIT}) : 1;
+  const long long room = units > (M > small ? 128 : 512) ? 1 : units > 0 ? 512 / units : 1;
+  const long long s = std::min({room, x->Lk / min_part, (long long)MAX_SPLIT});
   if (s > 1) {
     p.split_keys = (int)(((x->Lk + s - 1) / s + 63) / 64 * 64);
     p.nsplit = (x->Lk + p.split_keys - 1) / p.split_keys;
