@@ -1374,19 +1374,24 @@ Plan plan_forward(const gpn_attn_args_t* x) {
   }
   // Tiles of few rows also where those of many would leave half the CUs or more without work and these do not (4 x 512 rows
   // and keys, 8 heads of 64: 15 against 21 us).  Nearer a full card the four times as many reads of the keys cost more (3 x 777,
-  // 8 query and 2 key/value heads of 128: 43 against 28 us).  Wide fp32 heads apart, whose waves then find no room beside each
-  // other in LDS.
-  p.few = M <= small || (prob * ((M + big - 1) / big) <= 128 && prob * ((M + small - 1) / small) >= 256 && !(f32 && x->D > 64));
+  // 8 query and 2 key/value heads of 128: 43 against 28 us), but for narrow heads under `causal`, where one round of large tiles
+  // takes as long as its longest (3000 positions, 8 query and 2 key/value heads of 64: 29 against 56 us; of 128: 105 against 91).
+  // Wide fp32 heads apart, whose waves then find no room beside each other in LDS.
+  const long long large = prob * ((M + big - 1) / big), few_to = x->causal && !f32 && x->D <= 64 ? 256 : 128;
+  p.few = M <= small || (large <= few_to && prob * ((M + small - 1) / small) >= 256 && !(f32 && x->D > 64));
   p.bm = p.few ? small : big;
   p.tiles = (int)((M + p.bm - 1) / p.bm);
   // The card takes 512 workgroups (two per CU).  Few rows that leave half the room or more have their keys cut too, into parts
   // of min_part or more so that a part outweighs its share of the join (one query, 8 heads, 64 K keys: 64 parts 51 us, 5.3 TB/s;
   // twice as many workgroups for eight queries of uneven lengths 82 against 76 us).  So do tiles of many rows that leave half
   // the CUs without work; with more, what the join reads and writes costs what the parts gain (5 x 777, 8 query and 2 key/value
-  // heads of 64, 250 workgroups: 33 us in two parts, 23 in one).
+  // heads of 64, 250 workgroups: 33 us in two parts, 23 in one), but for long keys under `causal`, where the second part evens
+  // out what the tiles see (4096 positions, 8 heads of 128, 256 workgroups: 91 us in one part, 81 in two; 16 heads of 2 x 700
+  // positions 22 and 31 us).
   const long long units = prob * p.tiles, min_part = f32 ? 128 : 256;
   p.nsplit = 1, p.split_keys = x->Lk;
-  const long long room = units > (M > small ? 128 : 512) ? 1 : units > 0 ? 512 / units : 1;
+  const long long split_to = M <= small ? 512 : x->causal && x->Lk >= 2048 ? 256 : 128;
+  const long long room = units < 1 || units > split_to || (p.few && M > small) ? 1 : 512 / units;
   const long long s = std::min({room, x->Lk / min_part, (long long)MAX_SPLIT});
   if (s > 1) {
     p.split_keys = (int)(((x->Lk + s - 1) / s + 63) / 64 * 64);
