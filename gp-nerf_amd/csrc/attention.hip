@@ -463,26 +463,30 @@ struct Fwd {
   static constexpr size_t lds = 4 * TILE;  // two stages of keys and values
 };
 
-template <typename T, int DP, int NW, int KT>
-__global__ void __launch_bounds__(64 * NW, 2) k_attn_fwd(const AttnP a) {
+template <typename T, int DP, int NW, int WK, int KT>
+__global__ void __launch_bounds__(64 * NW * WK, 2) k_attn_fwd(const AttnP a) {
   using F = Fwd<T, DP, NW, KT>;
   using M = Mt<T>;
   using L = Lay<T, DP>;
+  constexpr int KW = KT / WK;  // the wave's share of a stage
   int pr, unit;
   if (!locate(a.B * a.Hkv, a.tiles * a.nsplit, pr, unit)) return;
-  const int split = unit / a.tiles, tile = a.tiles - 1 - (unit - split * a.tiles);  // causal: the longest tiles first
+  // causal: the longest tiles first; where all are on the card at once (two per CU), the second half in turn, shortest beside
+  // longest
+  const int split = unit / a.tiles, u = unit - split * a.tiles, most = WK == 2 ? (a.tiles + 1) / 2 : a.tiles;
+  const int tile = u < most ? a.tiles - 1 - u : u - most;
   const Prob p = problem(a, pr);
-  const int lane = threadIdx.x & 63, wave = wave_index(), n = lane & (M::TM - 1), h = lane / M::TM;
-  const Rows r = rows_of(a, p, tile * F::BM, tile * F::BM + wave * M::TM + n, F::BM, split);
-  clear_tail<T, DP>(attn_smem, 4 * KT, a.D, F::NTH);
+  const int lane = threadIdx.x & 63, wave = wave_index(), wm = wave % NW, wk = wave / NW, n = lane & (M::TM - 1), h = lane / M::TM;
+  const Rows r = rows_of(a, p, tile * F::BM, tile * F::BM + wm * M::TM + n, F::BM, split);
+  clear_tail<T, DP>(attn_smem, 4 * KT, a.D, F::NTH * WK);
 
   const T* kb = (const T*)a.k + p.b * a.sk.b + p.hk * a.sk.h;
   const T* vb = (const T*)a.v + p.b * a.sv.b + p.hk * a.sv.h;
   const unsigned base = lds_address(attn_smem);
   Keys<KT> keys = {a.key_mask ? a.key_mask + p.b * a.mask_sb : nullptr, r.kend, 0};
   const auto request = [&](int j0, unsigned long long bits, int buf) {
-    load_keys<T, DP, KT, NW>(kb, a.sk.l, a.D, j0, bits, base + buf * 2 * F::TILE, wave, lane);
-    load_keys<T, DP, KT, NW>(vb, a.sv.l, a.D, j0, bits, base + (buf * 2 + 1) * F::TILE, wave, lane);
+    load_keys<T, DP, KT, NW * WK>(kb, a.sk.l, a.D, j0, bits, base + buf * 2 * F::TILE, wave, lane);
+    load_keys<T, DP, KT, NW * WK>(vb, a.sv.l, a.D, j0, bits, base + (buf * 2 + 1) * F::TILE, wave, lane);
   };
   keys.fetch(r.kbeg, lane);
   unsigned long long bits = keys.bits(r.kbeg), next = 0;
@@ -502,11 +506,41 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_fwd(const AttnP a) {
     next = keys.bits(j0 + KT);
     keys.fetch(j0 + 2 * KT, lane);
     if (next) request(j0 + KT, next, buf ^ 1);
-    if (bits && !__all(r.lim < j0))
-      attend<T, DP, KT>(attn_smem + buf * 2 * F::TILE, attn_smem + (buf * 2 + 1) * F::TILE, qf, o, m, l, bits, j0, r.lim, a.c, lane);
+    const char* ks = attn_smem + buf * 2 * F::TILE + wk * KW * L::ROWB;
+    const unsigned long long mine = bits >> (wk * KW) & Keys<KW>::ALL;
+    if (mine && !__all(r.lim < j0 + wk * KW)) attend<T, DP, KW>(ks, ks + F::TILE, qf, o, m, l, mine, j0 + wk * KW, r.lim, a.c, lane);
     stage_done<0, true>();
   }
   l = col_sum<T>(l);
+  if constexpr (WK == 2) {  // the waves of the other half of every stage hand reference, sum and output over
+    float* mo = (float*)attn_smem + NW * L::MD * M::NC * 64;
+    fl4* x = (fl4*)attn_smem + wm * L::MD * (M::NC / 4) * 64 + lane;
+    if (wk) {
+      mo[wm * 64 + lane] = m, mo[(NW + wm) * 64 + lane] = l;
+#pragma unroll
+      for (int md = 0; md < L::MD; ++md)
+#pragma unroll
+        for (int q = 0; q < M::NC / 4; ++q) {
+          fl4 y;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = o[md][4 * q + e];
+          x[(md * (M::NC / 4) + q) * 64] = y;
+        }
+    }
+    __syncthreads();
+    if (wk) return;
+    const float m1 = mo[wm * 64 + lane], l1 = mo[(NW + wm) * 64 + lane], mm = fmaxf(m, m1), ms = mm == -INFINITY ? 0.f : mm;
+    const float f0 = exp2_((m - ms) * a.c), f1 = exp2_((m1 - ms) * a.c);
+    m = mm, l = l * f0 + l1 * f1;
+#pragma unroll
+    for (int md = 0; md < L::MD; ++md)
+#pragma unroll
+      for (int q = 0; q < M::NC / 4; ++q) {
+        const fl4 y = x[(md * (M::NC / 4) + q) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[md][4 * q + e] = o[md][4 * q + e] * f0 + y[e] * f1;
+      }
+  }
   if (!r.live) return;
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // a row without a key is zero
   const float l2 = l == 0.f ? -INFINITY : m * a.c + log2_(l);
@@ -785,7 +819,8 @@ __global__ void __launch_bounds__(64 * NW * WK, 2) k_attn_dq(const AttnP a) {
   static_assert(WK == 1 || WK == 2, "the join below is of two waves");
   int pr, unit;
   if (!locate(a.B * a.Hkv, a.tiles, pr, unit)) return;
-  const int tile = a.tiles - 1 - unit;
+  // longest tiles first; where all are on the card at once (two per CU), the second half in turn, shortest beside longest
+  const int most = NW == 2 ? (a.tiles + 1) / 2 : a.tiles, tile = unit < most ? a.tiles - 1 - unit : unit - most;
   const Prob p = problem(a, pr);
   const int lane = threadIdx.x & 63, wave = wave_index(), wm = wave % NW, wk = wave / NW, n = lane & (TM - 1), h = lane / TM;
   const Rows r = rows_of(a, p, tile * F::BM, tile * F::BM + wm * TM + n, F::BM, 0);
@@ -1353,46 +1388,57 @@ int launch(K kernel, const char* name, long long grid, int threads, size_t lds, 
   return GPN_OK;
 }
 
+// Two waves along the rows and two along the keys instead of four along the rows: twice as many workgroups of half the rows,
+// where one workgroup of the latter per CU takes all tiles, or two where tiles differ or heads are narrow: they fill the card and
+// even out.  (2048 causal positions, 8 heads: fp32 of 64, forward 84 -> 59 us, backward 214 -> 175; bf16 of 128, forward 45 -> 36.
+// 2 x 2000 causal, 8 fp32 heads of 32: 77 -> 49, 206 -> 160.)  With more, keys are read more often than that gains (3 x 1000, 16
+// heads of 128: 40 against 47, 131 against 140).
+bool is_mid(long long prob, long long M, bool f32, int D, bool causal) {
+  const long long large = prob * ((M + (f32 ? 63 : 127)) / (f32 ? 64 : 128));
+  return large <= (causal || D <= 64 ? 512 : 256);
+}
+
 // How a forward call is cut: rows per workgroup, keys per stage, splits of the keys.
 struct Plan {
   bool one_piece;  // few enough keys for one workgroup's registers
-  bool few;  // one tile of rows per problem: the waves of a workgroup share the rows and divide the keys
+  bool few;        // one tile of rows per workgroup, whose waves divide the keys
+  bool mid;        // two waves along the rows, two along the keys
   int bm, tiles, nsplit, split_keys;
 };
 
 Plan plan_forward(const gpn_attn_args_t* x) {
-  Plan p;
+  Plan p = {};
   const bool f32 = x->dtype == GPN_DT_F32;
   const long long M = (long long)x->Lq * (x->Hq / x->Hkv), prob = (long long)x->B * x->Hkv;
   const int big = f32 ? 64 : 128, small = f32 ? 16 : 32;
+  p.nsplit = 1, p.split_keys = x->Lk;
   p.one_piece = x->Lk <= (f32 && x->D > 64 ? 64 : 128);  // 64 KB of keys and values: two workgroups per CU
   if (p.one_piece) {  // as many waves as there are tiles of rows, four at most
-    p.few = false, p.nsplit = 1, p.split_keys = x->Lk;
     p.bm = M <= small ? small : M <= 2 * small ? 2 * small : 4 * small;
     p.tiles = (int)((M + p.bm - 1) / p.bm);
     return p;
   }
-  // Tiles of few rows also where those of many would leave half the CUs or more without work and these do not (4 x 512 rows
-  // and keys, 8 heads of 64: 15 against 21 us).  Nearer a full card the four times as many reads of the keys cost more (3 x 777,
-  // 8 query and 2 key/value heads of 128: 43 against 28 us), but for narrow heads under `causal`, where one round of large tiles
-  // takes as long as its longest (3000 positions, 8 query and 2 key/value heads of 64: 29 against 56 us; of 128: 105 against 91).
-  // Wide fp32 heads apart, whose waves then find no room beside each other in LDS.
-  const long long large = prob * ((M + big - 1) / big), few_to = x->causal && !f32 && x->D <= 64 ? 256 : 128;
-  p.few = M <= small || (large <= few_to && prob * ((M + small - 1) / small) >= 256 && !(f32 && x->D > 64));
-  p.bm = p.few ? small : big;
+  // Tiles of few rows also for narrow heads under `causal` whose tiles see anything from nothing to all keys and fill no more than
+  // the card: the finest cut evens out best (3000 positions, 8 query and 2 key/value heads of 64: 29 against 38 us; 2048, 8 heads:
+  // 21 against 28).  Fewer positions fill the card only where there are enough problems for larger tiles (4 x 1024, 8 heads: 23
+  // against 19).
+  const long long large = prob * ((M + big - 1) / big);
+  const bool steep = x->causal && !f32 && x->D <= 64 && x->Lq >= x->Lk / 2 && large <= (x->Lk >= 2048 ? 256 : 128) &&
+                     prob * ((M + small - 1) / small) >= 256;
+  p.few = M <= small || steep;
+  // wide fp32 heads, of which such a wave takes 16 keys at a time: only where tiles of many rows leave no room for parts of the keys
+  // (333 x 6 heads of 80, 1021 keys: 41 against 43 us)
+  p.mid = !p.few && is_mid(prob, M, f32, x->D, x->causal) && !(f32 && x->D > 64 && large <= 128);
+  p.bm = p.few ? small : p.mid ? big / 2 : big;
   p.tiles = (int)((M + p.bm - 1) / p.bm);
-  // The card takes 512 workgroups (two per CU).  Few rows that leave half the room or more have their keys cut too, into parts
-  // of min_part or more so that a part outweighs its share of the join (one query, 8 heads, 64 K keys: 64 parts 51 us, 5.3 TB/s;
-  // twice as many workgroups for eight queries of uneven lengths 82 against 76 us).  So do tiles of many rows that leave half
-  // the CUs without work; with more, what the join reads and writes costs what the parts gain (5 x 777, 8 query and 2 key/value
-  // heads of 64, 250 workgroups: 33 us in two parts, 23 in one), but for long keys under `causal`, where the second part evens
-  // out what the tiles see (4096 positions, 8 heads of 128, 256 workgroups: 91 us in one part, 81 in two; 16 heads of 2 x 700
-  // positions 22 and 31 us).
+  // The card takes 512 workgroups (two per CU).  Where there are half as many or fewer the keys are cut too, into parts of
+  // min_part or more so that a part outweighs its share of the join.  (One query, 8 heads, 64 K keys: 64 parts 51 us, 5.3 TB/s;
+  // twice as many workgroups for eight queries of uneven lengths 82 against 76 us.)  Workgroups of many rows that are more than
+  // half the CUs' number only where the keys are long or their products slow (1100 queries, 16 K keys, 8 heads of 128: 240 us in
+  // one part, 130 in two; fp32 2 x 400, 4 x 2 heads of 128, 1400 keys: 93 and 73; but 2 x 777, 8 query and 2 key/value heads of 64: 16, 21).
   const long long units = prob * p.tiles, min_part = f32 ? 128 : 256;
-  p.nsplit = 1, p.split_keys = x->Lk;
-  const long long split_to = M <= small ? 512 : x->causal && x->Lk >= 2048 ? 256 : 128;
-  const long long room = units < 1 || units > split_to || (p.few && M > small) ? 1 : 512 / units;
-  const long long s = std::min({room, x->Lk / min_part, (long long)MAX_SPLIT});
+  const long long split_to = M <= small ? 512 : steep ? 0 : (f32 && x->D > 64) || x->Lk >= 2048 ? 256 : 128;
+  const long long s = units < 1 || units > split_to ? 1 : std::min({512 / units, x->Lk / min_part, (long long)MAX_SPLIT});
   if (s > 1) {
     p.split_keys = (int)(((x->Lk + s - 1) / s + 63) / 64 * 64);
     p.nsplit = (x->Lk + p.split_keys - 1) / p.split_keys;
@@ -1461,8 +1507,14 @@ int forward_t(AttnP& a, const Plan& pl, hipStream_t st) {
     rc = launch(k_attn_few<T, DP, WK, KT>, "k_attn_few", grid, F::NTH, F::lds, st, a);
   } else {
     constexpr int KT = F32 && DP > 64 ? 32 : 64;  // two stages of 64 KB at most: two workgroups per CU
-    using F = Fwd<T, DP, 4, KT>;
-    rc = launch(k_attn_fwd<T, DP, 4, KT>, "k_attn_fwd", grid, F::NTH, F::lds, st, a);
+    if (pl.mid) {
+      using F = Fwd<T, DP, 2, KT>;
+      constexpr size_t join = 2 * (F::L::MD * Mt<T>::NC + 2) * 64 * 4;
+      rc = launch(k_attn_fwd<T, DP, 2, 2, KT>, "k_attn_fwd", grid, 256, std::max((size_t)F::lds, join), st, a);
+    } else {
+      using F = Fwd<T, DP, 4, KT>;
+      rc = launch(k_attn_fwd<T, DP, 4, 1, KT>, "k_attn_fwd", grid, F::NTH, F::lds, st, a);
+    }
   }
   if (rc || pl.nsplit == 1) return rc;
   const long long rows = (long long)a.B * a.Hkv * a.M;
@@ -1526,22 +1578,25 @@ int backward_t(AttnP& a, bool shrt, int nsplit, hipStream_t st) {
       return n <= 32 ? short_t<T, DP, 32>(a, st) : n <= 64 ? short_t<T, DP, 64>(a, st) : short_t<T, DP, 128>(a, st);
     }
   }
+  int rc;
   {
     constexpr int KT = F32 && DP > 64 ? 32 : 64;
-    using F = Fwd<T, DP, 4, KT>;
-    a.tiles = (a.M + F::BM - 1) / F::BM;
-    // Where one workgroup per CU takes all tiles, eight waves share a tile's keys: two waves to a SIMD either way.
-    constexpr size_t join = (size_t)4 * F::L::MD * Mt<T>::NC * 64 * 4;
-    const int rc = prob * a.tiles > 256
-                       ? launch(k_attn_dq<T, DP, 4, KT, 1>, "k_attn_dq", grid_of(prob, a.tiles), 256, F::lds, st, a)
-                       : launch(k_attn_dq<T, DP, 4, KT, 2>, "k_attn_dq", grid_of(prob, a.tiles), 512, std::max(F::lds, join), st, a);
+    if (is_mid(prob, a.M, F32, a.D, a.causal)) {
+      using F = Fwd<T, DP, 2, KT>;
+      constexpr size_t join = (size_t)2 * F::L::MD * Mt<T>::NC * 64 * 4;
+      a.tiles = (a.M + F::BM - 1) / F::BM;
+      rc = launch(k_attn_dq<T, DP, 2, KT, 2>, "k_attn_dq", grid_of(prob, a.tiles), 256, std::max((size_t)F::lds, join), st, a);
+    } else {
+      using F = Fwd<T, DP, 4, KT>;
+      a.tiles = (a.M + F::BM - 1) / F::BM;
+      rc = launch(k_attn_dq<T, DP, 4, KT, 1>, "k_attn_dq", grid_of(prob, a.tiles), 256, F::lds, st, a);
+    }
     if (rc) return rc;
   }
   a.tiles = (a.Lk + dkv_keys(F32) - 1) / dkv_keys(F32), a.nsplit = nsplit;
   const long long units = (long long)(a.causal ? (a.tiles + 1) / 2 : a.tiles) * nsplit, grid = grid_of(prob, units);
   // Pairs of waves per key tile keep the parts few where there are few tiles; with two workgroups for every CU in any case,
   // workgroups of four waves wait for each other less (4 x 4096 of 16 heads of 64: 1107 us for the backward in pairs, 1062).
-  int rc;
   if (!F32 && prob * units >= 512) rc = dkv_t<T, DP, F32 ? 2 : 1>(a, grid, st);
   else rc = dkv_t<T, DP, 2>(a, grid, st);
   if (rc || nsplit == 1) return rc;

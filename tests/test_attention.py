@@ -528,3 +528,23 @@ def test_groups_of_heads(dtype, G):
 def test_many_problems(dtype, shape, causal):
     """More problems than workgroups fit the card at once."""
     _run(*_inputs(dtype, *shape), causal=causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape,causal", [((6, 200, 300, 6, 3, 64), False), ((2, 1100, 2100, 4, 4, 24), True),
+                                          ((2, 1500, 2100, 4, 2, 40), True), ((4, 130, 700, 4, 2, 80), False),
+                                          ((5, 700, 200, 16, 16, 96), True), ((66, 140, 200, 8, 8, 16), False),
+                                          ((66, 260, 140, 4, 4, 112), False)], ids=str)
+def test_every_cut_of_masked_batches(dtype, shape, causal):
+    """Lengths, masks and starts with every way of cutting rows and keys: few rows, halves of tiles, whole tiles, parts."""
+    B, Lq, Lk = shape[:3]
+    q, k, v, do = _inputs(dtype, *shape)
+    g = torch.Generator().manual_seed(5)
+    lengths = torch.randint(0, Lk + 1, (B,), generator=g, dtype=torch.int32)
+    lengths[0] = Lk
+    lengths[-1] = 0
+    mask = torch.rand(B, Lk, generator=g) < 0.8
+    mask[0, :130] = False  # whole stages without a key
+    kw = dict(causal=True, q_start=(Lk - Lq + torch.arange(B, dtype=torch.int32) % 5 - 2).cuda()) if causal else {}
+    _run(q, k, v, do, lengths=lengths.cuda(), key_mask=mask.cuda(), **kw)
