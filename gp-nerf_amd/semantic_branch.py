@@ -6,8 +6,9 @@ Runs once per image on the rendered [1,512,h,w] feature image (about 8 GFLOP; SU
 plain torch module on the HIP device: conv / GroupNorm / bilinear resize are library ops, not part of
 the per-ray hot path that the HIP kernels of this package replace.  detectron2's `Conv2d(norm=...,
 activation=...)` is restated as conv -> GroupNorm(32,128) -> ReLU and fvcore's c2_msra_fill as
-kaiming_normal_(fan_out, relu).  The training-only distillation / depth-guided losses (:60-88) are
-out of scope (loss code) and raise.  The reference hard-codes a 120x160 feature image (:95); here
+kaiming_normal_(fan_out, relu).  The head's own training branch (:60-88: feature
+distillation, depth guidance) is out of scope and raises.  `distill_topk_loss` teaches class logits (the head's, or rows over
+a vocabulary) from a teacher's top entries, with its gradient.  The reference hard-codes a 120x160 feature image (:95); here
 the size is taken from the input (identical for 120x160).
 """
 import ctypes as C
