@@ -107,7 +107,7 @@ def _call(fn, name, backward, dev, *fields):
 
 def attention_forward(q, k, v, lengths=None, key_mask=None, causal=False, q_start=None, scale=None):
     """-> out [B, Lq, Hq, D] of q's type, lse [B, Hq, Lq] float32 (natural logarithm of the row's sum; -inf without a key).
-    scale: of the scores, positive (1 / sqrt(D) unless given).  No graph is recorded."""
+    scale: of the scores, from 1e-30 to 1e30 (1 / sqrt(D) unless given).  No graph is recorded."""
     head, keep = _args(q, k, v, lengths, key_mask, causal, q_start, scale)
     B, Lq, Hq, D = q.shape
     dev = q.device

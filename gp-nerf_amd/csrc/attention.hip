@@ -1475,7 +1475,7 @@ int check_args(const gpn_attn_args_t* x, const char* name) {
   GPN_REQUIRE(G <= 256 && (long long)x->Lq * G <= (1 << 24), "%s: %d queries x %d heads per key/value head", name, x->Lq, G);
   GPN_REQUIRE(x->Lk <= (1 << 30), "%s: %d keys", name, x->Lk);
   GPN_REQUIRE((long long)x->B * x->Hkv <= (1 << 24), "%s: %d batches x %d key/value heads", name, x->B, x->Hkv);
-  GPN_REQUIRE(x->scale > 0.f && x->scale < INFINITY, "%s: scale must be positive and finite", name);
+  GPN_REQUIRE(x->scale >= 1e-30f && x->scale <= 1e30f, "%s: scale must be between 1e-30 and 1e30", name);
   return GPN_OK;
 }
 

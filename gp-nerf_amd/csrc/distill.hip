@@ -539,7 +539,8 @@ int run(const gpn_distill_args_t* x, hipStream_t st, const char* name) {
   GPN_REQUIRE(x->N >= 0 && x->N <= INT_MAX, "%s: %lld rows", name, x->N);
   GPN_REQUIRE(x->C >= 1 && x->C <= (1 << 29), "%s: %d classes", name, x->C);
   GPN_REQUIRE(x->K >= 0 && x->K <= GPN_DISTILL_MAX_K, "%s: K must be in [0,%d] (got %d)", name, GPN_DISTILL_MAX_K, x->K);
-  GPN_REQUIRE(x->temperature > 0.f && x->temperature < INFINITY, "%s: temperature must be positive and finite", name);
+  // its square and its reciprocal stay far within fp32
+  GPN_REQUIRE(x->temperature >= 1e-12f && x->temperature <= 1e12f, "%s: temperature must be between 1e-12 and 1e12", name);
   GPN_REQUIRE(x->reduction >= GPN_RED_NONE && x->reduction <= GPN_RED_MEAN, "%s: unknown reduction %d", name, x->reduction);
   GPN_REQUIRE(x->logits || x->N == 0, "%s: null logits", name);
   GPN_REQUIRE((x->teacher && x->index) || x->K == 0 || x->N == 0, "%s: null teacher", name);

@@ -399,7 +399,7 @@ typedef struct {
   int dtype;                 /* GPN_DT_*: of q, k, v, out, dout, dq, dk, dv */
   int B, Lq, Lk, Hq, Hkv, D; /* Hq a multiple of Hkv; D a multiple of 8, at most GPN_ATTN_MAX_D */
   int causal;
-  float scale;               /* positive, finite */
+  float scale;               /* 1e-30 to 1e30 */
   const void *q, *k, *v;     /* [B,Lq,Hq,D], [B,Lk,Hkv,D] x 2: 16-byte aligned, contiguous along D, and strided: */
   long long q_stride[3], k_stride[3], v_stride[3]; /* elements between batches, positions, heads (multiples of 16 bytes; 0 is
                                                       a broadcast) */
@@ -443,7 +443,7 @@ typedef struct {
   int index_bytes;            /* 4 or 8: index is int32 or int64 */
   int C, K;                   /* classes (at most 2^29), teacher entries per row (at most GPN_DISTILL_MAX_K) */
   int reduction;              /* GPN_RED_* */
-  float temperature;
+  float temperature;          /* 1e-12 to 1e12 */
   float grad_scale;           /* gpn_distill_step: dlogits is the gradient of grad_scale * loss */
   long long N;
   const void* logits;         /* element (n, c) at n * row_stride + c * class_stride; one of the two strides is 1 */

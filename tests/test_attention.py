@@ -98,6 +98,15 @@ def test_c_entry_refuses(bad, text):
     assert L.gpn_attn_backward(ctypes.byref(_fake(**bad)), None) == -1
 
 
+@pytest.mark.parametrize("scale", [1e-38, 3e38])
+def test_c_entry_refuses_scales_that_overflow(scale):
+    from gp_nerf_amd import _lib
+    L = _lib.lib()
+    for fn in (L.gpn_attn_forward, L.gpn_attn_backward):
+        assert fn(ctypes.byref(_fake(scale=scale)), None) == -1
+        assert b"scale must be between" in L.gpn_last_error()
+
+
 def test_c_entry_refuses_missing_workspace_and_gradients():
     from gp_nerf_amd import _lib
     L = _lib.lib()

@@ -112,6 +112,15 @@ def test_c_entry_refuses(bad, text):
         assert text in L.gpn_last_error().decode()
 
 
+@pytest.mark.parametrize("temperature", [1e-20, 1e20, -1.0, float("nan")])
+def test_c_entry_refuses_temperatures_whose_square_is_lost(temperature):
+    from gp_nerf_amd import _lib
+    L = _lib.lib()
+    for fn in (L.gpn_distill_forward, L.gpn_distill_backward, L.gpn_distill_step):
+        assert fn(ctypes.byref(_fake(temperature=temperature)), None) == -1
+        assert b"temperature must be between" in L.gpn_last_error()
+
+
 def test_c_entry_refuses_missing_outputs():
     from gp_nerf_amd import _lib
     L = _lib.lib()
