@@ -959,7 +959,7 @@ struct Dkv {
   static constexpr size_t stage_bytes = v_at + (VL ? BN * L::ROWB : 0);
   static constexpr size_t join_bytes = WR > 1 ? (size_t)WN * 2 * L::MD * M::NC * 64 * 4 : 0;
   static constexpr size_t lds = stage_bytes > join_bytes ? stage_bytes : join_bytes;
-  static constexpr int LOADS = 2 * Dma<T, DP, RB, NW>::COUNT;  // of a wave per stage: this many, one more, or (no rows for it) none
+  static constexpr int LOADS = 2 * Dma<T, DP, RB, NW>::COUNT;  // of a wave per stage: this many or more, or (no rows for it) none
 };
 
 template <typename T, int DP, int WN, int WR>
@@ -1014,11 +1014,17 @@ __global__ void __launch_bounds__(64 * WN * WR, 2) k_attn_dkv(const AttnP a) {
       Dm::rows([&](int r) { return at(q0, a.sq, r); }, a.D, to, wave, lane);
       Dm::rows([&](int r) { return at(d0, a.sdo, r); }, a.D, to + F::TILE, wave, lane);
     }
-    if (wave < 2 && lane < RB) {
+    // the rows' statistics, by waves that bring rows too: the wait for a stage counts loads, LOADS or more of them per stage
+    const auto bring = [&](int which) {
       const int r = r0 + lane;
-      const float* src = wave ? (r < a.M ? a.delta + (long long)pr * a.M + r : (const float*)attn_zero)
-                              : (r < a.M ? a.lse2 + (long long)pr * a.M + r : &attn_inf);
-      dma4(src, base + F::stats_at + buf * 512 + wave * 256);
+      const float* src = which ? (r < a.M ? a.delta + (long long)pr * a.M + r : (const float*)attn_zero)
+                               : (r < a.M ? a.lse2 + (long long)pr * a.M + r : &attn_inf);
+      dma4(src, base + F::stats_at + buf * 512 + which * 256);
+    };
+    if constexpr (RB > Dm::RPI) {
+      if (wave < 2 && lane < RB) bring(wave);
+    } else if (wave == 0 && lane < RB) {
+      bring(0), bring(1);
     }
   };
 

@@ -557,3 +557,11 @@ def test_every_cut_of_masked_batches(dtype, shape, causal):
     mask[0, :130] = False  # whole stages without a key
     kw = dict(causal=True, q_start=(Lk - Lq + torch.arange(B, dtype=torch.int32) % 5 - 2).cuda()) if causal else {}
     _run(q, k, v, do, lengths=lengths.cuda(), key_mask=mask.cuda(), **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_narrow_heads_over_many_stages(dtype, causal):
+    """Heads of 16, whose stages of rows one wave brings alone."""
+    _run(*_inputs(dtype, 33, 700, 260, 16, 8, 16), causal=causal)
