@@ -31,6 +31,8 @@ MAX_D = 128
 
 def _rows(t):
     """(tensor the kernels can read, its strides between batches, positions and heads): 16-byte rows, contiguous along D."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:  # (D is a multiple of 8)
+        return t, t.stride()[:3]
     per = 16 // t.element_size()
     for copy in (None, torch.Tensor.contiguous, torch.Tensor.clone):
         if copy is not None:
@@ -109,11 +111,9 @@ def attention_forward(q, k, v, lengths=None, key_mask=None, causal=False, q_star
     """-> out [B, Lq, Hq, D] of q's type, lse [B, Hq, Lq] float32 (natural logarithm of the row's sum; -inf without a key).
     scale: of the scores, from 1e-30 to 1e30 (1 / sqrt(D) unless given).  No graph is recorded."""
     head, keep = _args(q, k, v, lengths, key_mask, causal, q_start, scale)
-    B, Lq, Hq, D = q.shape
-    dev = q.device
-    out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=dev)
-    lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=dev)
-    _call(_lib.lib().gpn_attn_forward, "gpn_attn_forward", 0, dev, *head, out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0, 0, 0)
+    out = q.new_empty(q.shape)
+    lse = q.new_empty((head[1], head[4], head[2]), dtype=torch.float32)
+    _call(_lib.lib().gpn_attn_forward, "gpn_attn_forward", 0, q.device, *head, out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, 0, 0, 0)
     return out, lse
 
 
@@ -131,7 +131,7 @@ def attention_backward(dout, q, k, v, out, lse, lengths=None, key_mask=None, cau
     if not out.is_contiguous() or out.data_ptr() % 16:
         out = out.clone(memory_format=torch.contiguous_format)
     lse = lse.contiguous()
-    dq, dk, dv = (torch.empty(t.shape, dtype=dt, device=dev) for t in (q, k, v))
+    dq, dk, dv = q.new_empty(shape), k.new_empty(k.shape), v.new_empty(v.shape)
     _call(_lib.lib().gpn_attn_backward, "gpn_attn_backward", 1, dev, *head, out.data_ptr(), lse.data_ptr(), dout.data_ptr(), *sdo,
           dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
     return dq, dk, dv
