@@ -51,12 +51,15 @@ MAX_TEACHER_ENTRIES = 256
 def _as_rows(x, name):
     """[N, C] as it is; an image [1, C, H, W] or [C, H, W] as the [H*W, C] view of its planes."""
     if isinstance(x, torch.Tensor):
+        if x.dim() == 2:
+            return x
+        if x.dim() in (3, 4) and x.is_contiguous() and x.numel() and x.shape[:-3] in ((), (1,)):
+            c, h, w = x.shape[-3:]
+            return x.as_strided((h * w, c), (1, h * w))
         if x.dim() == 4 and x.shape[0] == 1:
             x = x[0]
         if x.dim() == 3:
-            x = x.flatten(1).t()
-        if x.dim() == 2:
-            return x
+            return x.flatten(1).t()
     raise ValueError("%s: expected [N, classes], [classes, H, W] or [1, classes, H, W]" % name)
 
 
@@ -99,9 +102,9 @@ def _distill_gradient(z, planes, logits):
     """Memory for dlogits as the logits lie (class planes or rows) -> it in the logits' shape, (address, strides)."""
     N, Cn = z.shape
     if planes:
-        d = torch.empty((Cn, N), dtype=z.dtype, device=z.device)
+        d = z.new_empty((Cn, N))
         return d.t() if logits.dim() == 2 else d.view(logits.shape), (d.data_ptr(), 1, N)
-    d = torch.empty((N, Cn), dtype=z.dtype, device=z.device)
+    d = z.new_empty((N, Cn))
     return d if logits.dim() == 2 else d.t().reshape(logits.shape), (d.data_ptr(), Cn, 1)
 
 
