@@ -1485,21 +1485,26 @@ int check_args(const gpn_attn_args_t* x, const char* name) {
   return GPN_OK;
 }
 
-int check_tensor(const void* p, const long long* s, int size, const char* what, const char* name) {
+// Strides of batches, positions and heads; nothing lies a stride away along a dimension of one, so that stride counts as 0,
+// whatever a slice of a larger tensor has there.
+Strides strides(const long long* s, int B, int L, int H) { return Strides{B > 1 ? s[0] : 0, L > 1 ? s[1] : 0, H > 1 ? s[2] : 0}; }
+Strides query_strides(const gpn_attn_args_t* x, const long long* s) { return strides(s, x->B, x->Lq, x->Hq); }
+Strides key_strides(const gpn_attn_args_t* x, const long long* s) { return strides(s, x->B, x->Lk, x->Hkv); }
+
+int check_tensor(const void* p, int size, const char* what, const char* name, Strides s = {}) {
   GPN_REQUIRE(p, "%s: null %s", name, what);
   GPN_REQUIRE(((size_t)p & 15) == 0, "%s: %s is not 16-byte aligned", name, what);
-  for (int i = 0; s && i < 3; ++i)
-    GPN_REQUIRE(s[i] >= 0 && s[i] * size % 16 == 0, "%s: stride %lld of %s is not a multiple of 16 bytes", name, s[i], what);
+  for (const long long x : {s.b, s.l, s.h})
+    GPN_REQUIRE(x >= 0 && x * size % 16 == 0, "%s: stride %lld of %s is not a multiple of 16 bytes", name, x, what);
   return GPN_OK;
 }
-
-Strides strides(const long long* s) { return Strides{s[0], s[1], s[2]}; }
 
 AttnP fill(const gpn_attn_args_t* x) {
   AttnP a = {};
   a.q = x->q, a.k = x->k, a.v = x->v, a.dout = x->dout;
   a.out = x->out, a.dq = x->dq, a.dk = x->dk, a.dv = x->dv;
-  a.sq = strides(x->q_stride), a.sk = strides(x->k_stride), a.sv = strides(x->v_stride), a.sdo = strides(x->dout_stride);
+  a.sq = query_strides(x, x->q_stride), a.sdo = query_strides(x, x->dout_stride);
+  a.sk = key_strides(x, x->k_stride), a.sv = key_strides(x, x->v_stride);
   a.lse = x->lse, a.lengths = x->lengths, a.q_start = x->causal ? x->q_start : nullptr, a.key_mask = x->key_mask;
   a.mask_sb = x->key_mask_stride;
   a.B = x->B, a.Lq = x->Lq, a.Lk = x->Lk, a.Hq = x->Hq, a.Hkv = x->Hkv, a.D = x->D;
@@ -1574,7 +1579,9 @@ int short_t(const AttnP& a, hipStream_t st) {
 bool is_near(const gpn_attn_args_t* x) {
   const long long m = 1 << 20;
   bool near = (long long)x->Hq * x->D < m;
-  for (int i = 1; i < 3; ++i) near &= x->q_stride[i] < m && x->k_stride[i] < m && x->v_stride[i] < m && x->dout_stride[i] < m;
+  for (const Strides& s : {query_strides(x, x->q_stride), query_strides(x, x->dout_stride), key_strides(x, x->k_stride),
+                           key_strides(x, x->v_stride)})
+    near &= s.l < m && s.h < m;
   return near;
 }
 
@@ -1670,12 +1677,12 @@ extern "C" int gpn_attn_forward(const gpn_attn_args_t* x, gpn_stream_t stream) {
   if (int rc = check_args(x, name)) return rc;
   if (x->B == 0 || x->Lq == 0) return GPN_OK;
   const int size = x->dtype == GPN_DT_F32 ? 4 : 2;
-  if (int rc = check_tensor(x->q, x->q_stride, size, "q", name)) return rc;
+  if (int rc = check_tensor(x->q, size, "q", name, query_strides(x, x->q_stride))) return rc;
   if (x->Lk > 0) {
-    if (int rc = check_tensor(x->k, x->k_stride, size, "k", name)) return rc;
-    if (int rc = check_tensor(x->v, x->v_stride, size, "v", name)) return rc;
+    if (int rc = check_tensor(x->k, size, "k", name, key_strides(x, x->k_stride))) return rc;
+    if (int rc = check_tensor(x->v, size, "v", name, key_strides(x, x->v_stride))) return rc;
   }
-  if (int rc = check_tensor(x->out, nullptr, size, "out", name)) return rc;
+  if (int rc = check_tensor(x->out, size, "out", name)) return rc;
   GPN_REQUIRE(x->lse, "%s: null lse", name);
   const Plan pl = plan_forward(x);
   const size_t need = gpn_attn_workspace_bytes(x, 0);
@@ -1698,17 +1705,17 @@ extern "C" int gpn_attn_backward(const gpn_attn_args_t* x, gpn_stream_t stream) 
   if (x->B == 0 || (x->Lq == 0 && x->Lk == 0)) return GPN_OK;
   const int size = x->dtype == GPN_DT_F32 ? 4 : 2;
   if (x->Lq > 0) {
-    if (int rc = check_tensor(x->q, x->q_stride, size, "q", name)) return rc;
-    if (int rc = check_tensor(x->dout, x->dout_stride, size, "dout", name)) return rc;
-    if (int rc = check_tensor(x->out, nullptr, size, "out", name)) return rc;
-    if (int rc = check_tensor(x->dq, nullptr, size, "dq", name)) return rc;
+    if (int rc = check_tensor(x->q, size, "q", name, query_strides(x, x->q_stride))) return rc;
+    if (int rc = check_tensor(x->dout, size, "dout", name, query_strides(x, x->dout_stride))) return rc;
+    if (int rc = check_tensor(x->out, size, "out", name)) return rc;
+    if (int rc = check_tensor(x->dq, size, "dq", name)) return rc;
     GPN_REQUIRE(x->lse, "%s: null lse", name);
   }
   if (x->Lk > 0) {
-    if (int rc = check_tensor(x->k, x->k_stride, size, "k", name)) return rc;
-    if (int rc = check_tensor(x->v, x->v_stride, size, "v", name)) return rc;
-    if (int rc = check_tensor(x->dk, nullptr, size, "dk", name)) return rc;
-    if (int rc = check_tensor(x->dv, nullptr, size, "dv", name)) return rc;
+    if (int rc = check_tensor(x->k, size, "k", name, key_strides(x, x->k_stride))) return rc;
+    if (int rc = check_tensor(x->v, size, "v", name, key_strides(x, x->v_stride))) return rc;
+    if (int rc = check_tensor(x->dk, size, "dk", name)) return rc;
+    if (int rc = check_tensor(x->dv, size, "dv", name)) return rc;
   }
   const size_t need = gpn_attn_workspace_bytes(x, 1);
   GPN_REQUIRE(x->workspace_bytes >= need && (need == 0 || x->workspace), "%s: workspace of %zu bytes, %zu needed", name,

@@ -402,7 +402,7 @@ typedef struct {
   float scale;               /* 1e-30 to 1e30 */
   const void *q, *k, *v;     /* [B,Lq,Hq,D], [B,Lk,Hkv,D] x 2: 16-byte aligned, contiguous along D, and strided: */
   long long q_stride[3], k_stride[3], v_stride[3]; /* elements between batches, positions, heads (multiples of 16 bytes; 0 is
-                                                      a broadcast) */
+                                                      a broadcast; anything along a dimension of one) */
   const int32_t* lengths;    /* [B] number of keys of each batch, or NULL: Lk */
   const uint8_t* key_mask;   /* [B,Lk] 0 = hidden, or NULL */
   long long key_mask_stride; /* bytes between its rows */

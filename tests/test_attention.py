@@ -565,3 +565,64 @@ def test_every_cut_of_masked_batches(dtype, shape, causal):
 def test_narrow_heads_over_many_stages(dtype, causal):
     """Heads of 16, whose stages of rows one wave brings alone."""
     _run(*_inputs(dtype, 33, 700, 260, 16, 8, 16), causal=causal)
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("at,single", [(0, dict(B=1)), (1, dict(Lq=1)), (1, dict(Lk=1)), (2, dict(Hq=1, Hkv=1)), (2, dict(Hkv=1))], ids=str)
+def test_c_entry_takes_any_stride_of_one_batch_position_or_head(name, at, single):
+    """No element lies a stride away along a dimension of one.  The call then stops at its missing workspace, before a launch."""
+    from gp_nerf_amd import _lib
+    L = _lib.lib()
+    alone = {"q": "Lq" in single or "Hq" in single, "k": "Lk" in single or "Hkv" in single}
+    alone = alone["q" if name in ("q", "dout") else "k"] or at == 0
+    for big in (2565, 1 << 40, -3):
+        sizes = dict(dict(Lq=300, Lk=300), **single)
+        strides = [512, 64, 16]
+        strides[at] = big
+        bad = _fake(**sizes, **{name + "_stride": tuple(strides)})
+        assert L.gpn_attn_backward(ctypes.byref(bad), None) == -1
+        text = L.gpn_last_error().decode()
+        assert "workspace" in text if alone or (big > 0 and big % 8 == 0) else "stride" in text, text
+        if name != "dout" and "Lk" not in single:
+            few = _fake(**dict(sizes, Lq=1, Lk=1 << 16), **{name + "_stride": tuple(strides)})  # (keys in parts)
+            assert L.gpn_attn_forward(ctypes.byref(few), None) == -1
+            text = L.gpn_last_error().decode()
+            one = alone or (at == 1 and name == "q")
+            assert "workspace" in text if one or (big > 0 and big % 8 == 0) else "stride" in text, text
+
+
+def test_strides_of_single_dimensions_do_not_choose_the_kernel():
+    """Gradients of short sequences need no workspace unless rows lie far apart."""
+    from gp_nerf_amd import _lib
+    L = _lib.lib()
+    far = (1 << 24, 1 << 24, 16)
+    assert L.gpn_attn_workspace_bytes(ctypes.byref(_fake()), 1) == 0
+    assert L.gpn_attn_workspace_bytes(ctypes.byref(_fake(q_stride=far)), 1) > 0
+    assert L.gpn_attn_workspace_bytes(ctypes.byref(_fake(Lq=1, q_stride=far, dout_stride=far)), 1) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 5, 9, 4, 2, 64), (3, 1, 1, 2, 2, 16), (2, 40, 70, 1, 1, 32), (1, 1, 300, 8, 8, 64),
+                                   (1, 200, 1, 1, 1, 128)], ids=str)
+def test_single_batches_positions_and_heads_of_any_pitch(dtype, shape):
+    """Dimensions of one element, as slices of larger tensors have them: their strides fit no alignment."""
+    x = _inputs(dtype, *shape)
+    want = _both(*x)
+
+    def odd(t, pitch):  # the same elements; dimensions of one get an odd stride
+        s = [p if n > 1 else pitch for n, p in zip(t.shape[:3], t.stride()[:3])]
+        return t.as_strided(t.shape, (*s, 1))
+
+    for pitch in (1027, 3, 2 ** 21 + 1):
+        got = _both(*(odd(t, pitch) for t in x))
+        for n in want:
+            assert torch.equal(want[n], got[n]), n
+    B, Lk, Hkv, D = x[1].shape
+    cache = torch.zeros(3, Lk * Hkv * D + 3, dtype=x[1].dtype).cuda()  # one batch of a buffer with an odd pitch
+    cache[0, :Lk * Hkv * D] = x[1][0].flatten()
+    k = cache[:, :Lk * Hkv * D].view(3, Lk, Hkv, D)[:1]
+    got = _both(x[0][:1], k, x[2][:1], x[3][:1])
+    want = _both(*(t[:1].contiguous() for t in x))
+    for n in want:
+        assert torch.equal(want[n], got[n]), n
