@@ -1345,6 +1345,10 @@ __global__ void __launch_bounds__(64 * MB / Mt<T>::TM, 2) k_attn_short(const Att
       for (; r0 < x1; r0 += TM) rows(r0, x0, std::false_type());
     }
     if (half == F::HALVES - 1 && key < a.Lk) {
+      if (!seen) {  // a hidden key's gradients are zero: its probabilities are, but not their products with what overflowed
+#pragma unroll
+        for (int md = 0; md < MD; ++md) dk[md] = dv[md] = (typename M::Acc)(0.f);
+      }
       const long long g0 = ((long long)p.b * a.Lk * a.Hkv + p.hk) * a.D;
       const unsigned at = (unsigned)(key * a.Hkv * a.D);
       store_cols<T, T, MD>(dk, a.scale, (T*)a.dk + g0 + at, a.D, h);

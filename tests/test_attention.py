@@ -626,3 +626,21 @@ def test_single_batches_positions_and_heads_of_any_pitch(dtype, shape):
     want = _both(*(t[:1].contiguous() for t in x))
     for n in want:
         assert torch.equal(want[n], got[n]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 20, 30, 2, 2, 16), (2, 64, 64, 4, 2, 32), (2, 60, 128, 2, 1, 24), (2, 128, 100, 2, 2, 16),
+                                   (2, 30, 70, 2, 1, 128), (2, 300, 200, 2, 2, 64)], ids=str)
+def test_gradients_of_hidden_keys_are_zero_under_overflown_ones(dtype, shape):
+    """A gradient that overflowed, or a query that is NaN, reaches no key that lengths or key_mask hide."""
+    B, Lq, Lk = shape[:3]
+    q, k, v, do = _inputs(dtype, *shape)
+    mask = torch.ones(B, Lk, dtype=torch.bool).cuda()
+    mask[:, 1::3] = False
+    lengths = torch.tensor([Lk, Lk // 2], dtype=torch.int32).cuda()
+    hide = ~(mask & (torch.arange(Lk).cuda() < lengths[:, None]))
+    do[0, 2, 0, 3] = float("inf")
+    q[1, 1, 1, 5] = float("nan")
+    got = _both(q, k, v, do, lengths=lengths, key_mask=mask)
+    assert not bool(got["dk"][hide].any()) and not bool(got["dv"][hide].any())
