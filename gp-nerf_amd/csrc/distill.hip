@@ -95,10 +95,10 @@ __device__ __forceinline__ void merge(float& m, float& l, float m2, float l2, fl
   m = M;
 }
 
-// gradient's factor of a row
-__device__ __forceinline__ float row_factor(const DistP& a, long long row) {
+// gradient's factor of a row of weight w
+__device__ __forceinline__ float row_factor(const DistP& a, long long row, float w) {
   const float g = a.dloss ? a.dloss[a.dloss_rows ? row : 0] : 1.f;
-  return g * a.grad_scale * a.T * (a.w ? a.w[row] : 1.f);
+  return g * a.grad_scale * a.T * w;
 }
 
 // ---------------------------------------------------------------------------------------------------------- rows
@@ -192,7 +192,8 @@ __global__ void __launch_bounds__(NT, CH > 8 ? 4 : 6) k_distill_rows(const DistP
     for (int w = 1; w < NW; ++w) merge(m, l, sred[w], sred[NW + w], a.c);
   }
   const float mt = sstat[0], lt = sstat[1];
-  const bool empty = !(lt > 0.f) && lt == lt;  // no entry at all
+  const float wt = a.w ? a.w[row] : 1.f;
+  const bool empty = wt == 0.f || (!(lt > 0.f) && lt == lt);  // left out, or no entry at all
   const float lt2 = log2_(lt);
   float l2;
   if (MODE == BWD) m = 0.f, l2 = a.lse_in[row] * LOG2E;
@@ -207,13 +208,13 @@ __global__ void __launch_bounds__(NT, CH > 8 ? 4 : 6) k_distill_rows(const DistP
 #pragma unroll
     for (int d = 32; d; d >>= 1) loss += __shfl_xor(loss, d);
     if (lane == 0) {
-      a.loss_rows[row] = empty ? 0.f : loss * LN2 * a.T * a.T * (a.w ? a.w[row] : 1.f);
+      a.loss_rows[row] = empty ? 0.f : loss * LN2 * a.T * a.T * wt;
       if (MODE == FWD) a.lse[row] = (m * a.c + l2) * LN2;
     }
   }
   if (MODE == FWD) return;
 
-  const float f = row_factor(a, row);
+  const float f = row_factor(a, row, wt);
   const float inv = MODE == BWD ? 0.f : 1.f / l, fi = f * inv;
   const auto prob = [&](float x) {
     const float u = (x - m) * a.c;
@@ -382,7 +383,8 @@ __global__ void __launch_bounds__(256) k_distill_planes(const DistP a) {
         for (int k = 0; k < a.K; ++k)
           if (entry(k) >= 0) merge(mt[v], lt, logit(k), 1.f, a.c);
       }
-      empty[v] = !(lt > 0.f) && lt == lt;
+      const float wt = a.w ? a.w[row] : 1.f;
+      empty[v] = wt == 0.f || (!(lt > 0.f) && lt == lt);  // left out, or no entry at all
       lt2[v] = log2_(lt);
       if (MODE == BWD) m[v] = 0.f, l2[v] = a.lse_in[row] * LOG2E;
       else l2[v] = log2_(l[v]);
@@ -401,12 +403,12 @@ __global__ void __launch_bounds__(256) k_distill_planes(const DistP a) {
         } else {
           for (int k = 0; k < a.K; ++k) add(k);
         }
-        loss = empty[v] ? 0.f : loss * LN2 * a.T * a.T * (a.w ? a.w[row] : 1.f);
+        loss = empty[v] ? 0.f : loss * LN2 * a.T * a.T * wt;
         if (a.loss_each) a.loss_rows[row] = loss;
         total += loss;
         if (MODE == FWD) a.lse[row] = (m[v] * a.c + l2[v]) * LN2;
       }
-      if (MODE != FWD) f[v] = row_factor(a, row), fi[v] = MODE == BWD ? 0.f : f[v] * (1.f / l[v]);
+      if (MODE != FWD) f[v] = row_factor(a, row, wt), fi[v] = MODE == BWD ? 0.f : f[v] * (1.f / l[v]);
     }
     if (MODE != FWD) {
       const auto grad = [&](float x, int v) {

@@ -452,7 +452,7 @@ typedef struct {
   long long teacher_stride[2];
   const void* index;          /* [N,K] with any strides */
   long long index_stride[2];
-  const float* row_weight;    /* [N] or NULL: 1 */
+  const float* row_weight;    /* [N] or NULL: 1.  A row of weight 0 is left out like one without an entry */
   float* loss_rows;           /* [N]: the rows' losses for GPN_RED_NONE, else scratch of forward and step */
   float* loss;                /* [1]: their sum or mean (reduction other than none) */
   float* lse;                 /* [N], written by forward, read by backward: log sum exp(z / T) */

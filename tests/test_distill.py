@@ -368,3 +368,31 @@ def test_ray_attention_under_a_distilled_head():
     assert abs(float(got.detach()) - float(want.detach())) <= tol * abs(float(want.detach()))
     for a, b in zip(own, ref):
         assert float((a.grad.cpu().double() - b.grad).abs().max()) <= tol * float(b.grad.abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("planes,C,K", [(False, 30, 6), (False, 1500, 6), (False, 140000, 6), (True, 30, 6), (True, 50, 6), (True, 40, 12)])
+def test_rows_of_weight_zero_may_hold_anything(dtype, planes, C, K):
+    """They count as rows without an entry: the others' results do not change by a bit."""
+    from gp_nerf_amd import semantic_branch as S
+    z, t, idx = _inputs(dtype, 10, C, K, planes=planes)
+    w = torch.linspace(0.5, 2, 10).cuda()
+    out = [1, 2, 4, 5, 9]
+    w[out] = torch.tensor([0.0, -0.0, 0.0, 0.0, 0.0]).cuda()
+    clean = z.clone(), t.clone()
+    z[1] = float("nan")
+    z[2, 3] = float("inf")
+    z[4, idx[4, 1]] = -float("inf")   # a class of the teacher's that the student rules out
+    t[5, 2] = float("nan")
+    t[9] = float("inf")
+    for red in ("none", "sum", "mean"):
+        up = torch.full((10,) if red == "none" else (), 1.5, device="cuda")
+        got, want = [], []
+        for zz, tt, to in ((z, t, got), (*clean, want)):
+            loss, lse = S.distill_topk_forward(zz, tt, idx, 0.9, w, red)
+            to += [loss, S.distill_topk_backward(up, zz, tt, idx, lse, 0.9, w, red), *S.distill_topk_step(zz, tt, idx, 0.9, w, red)]
+        for a, b in zip(got, want):
+            assert bool(a.isfinite().all()) and torch.equal(a, b), red
+        assert not bool(got[1][out].any()) and not bool(got[3][out].any())
+        assert red != "none" or not bool(got[0][out].any())
