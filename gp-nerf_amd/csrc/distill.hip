@@ -95,6 +95,10 @@ __device__ __forceinline__ void merge(float& m, float& l, float m2, float l2, fl
   m = M;
 }
 
+// log sum exp(z / T) from the maximum and log2 of the sum relative to it.  (m c alone would overflow for logits near the type's
+// limits, whose log-sum-exp is a number.)
+__device__ __forceinline__ float row_lse(const DistP& a, float m, float l2) { return m / a.T + l2 * LN2; }
+
 // gradient's factor of a row of weight w
 __device__ __forceinline__ float row_factor(const DistP& a, long long row, float w) {
   const float g = a.dloss ? a.dloss[a.dloss_rows ? row : 0] : 1.f;
@@ -209,7 +213,7 @@ __global__ void __launch_bounds__(NT, CH > 8 ? 4 : 6) k_distill_rows(const DistP
     for (int d = 32; d; d >>= 1) loss += __shfl_xor(loss, d);
     if (lane == 0) {
       a.loss_rows[row] = empty ? 0.f : loss * LN2 * a.T * a.T * wt;
-      if (MODE == FWD) a.lse[row] = (m * a.c + l2) * LN2;
+      if (MODE == FWD) a.lse[row] = row_lse(a, m, l2);
     }
   }
   if (MODE == FWD) return;
@@ -406,7 +410,7 @@ __global__ void __launch_bounds__(256) k_distill_planes(const DistP a) {
         loss = empty[v] ? 0.f : loss * LN2 * a.T * a.T * wt;
         if (a.loss_each) a.loss_rows[row] = loss;
         total += loss;
-        if (MODE == FWD) a.lse[row] = (m[v] * a.c + l2[v]) * LN2;
+        if (MODE == FWD) a.lse[row] = row_lse(a, m[v], l2[v]);
       }
       if (MODE != FWD) f[v] = row_factor(a, row, wt), fi[v] = MODE == BWD ? 0.f : f[v] * (1.f / l[v]);
     }

@@ -396,3 +396,18 @@ def test_rows_of_weight_zero_may_hold_anything(dtype, planes, C, K):
             assert bool(a.isfinite().all()) and torch.equal(a, b), red
         assert not bool(got[1][out].any()) and not bool(got[3][out].any())
         assert red != "none" or not bool(got[0][out].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("planes", [False, True])
+def test_log_sum_exp_of_the_largest_logits(dtype, planes):
+    """Logits at the ends of their type have a log-sum-exp that fp32 holds."""
+    from gp_nerf_amd import semantic_branch as S
+    z, t, idx = _inputs(dtype, 6, 40, 4, planes=planes)
+    top = torch.finfo(TYPES[dtype]).max
+    z[0], z[1], z[2, 3], z[3] = -top, top, top, -0.75 * top
+    for T in (1.0, 3.0):
+        lse = S.distill_topk_forward(z, t, idx, T)[1]
+        assert bool(lse.isfinite().all())
+        _near("lse", lse, oracle.distill(z, t, idx, T, bits=z.dtype))
