@@ -411,3 +411,19 @@ def test_log_sum_exp_of_the_largest_logits(dtype, planes):
         lse = S.distill_topk_forward(z, t, idx, T)[1]
         assert bool(lse.isfinite().all())
         _near("lse", lse, oracle.distill(z, t, idx, T, bits=z.dtype))
+
+
+@pytest.mark.parametrize("offset", [-1e9, 1e16, -3e38, "cold"])
+def test_oracle_does_not_depend_on_a_common_offset(offset):
+    """Differences of a row's logits that 64 bits hold come back from it whatever they are added to; its bounds stay finite."""
+    z, t, idx = _inputs("fp32", 5, 60, 4, dev="cpu")
+    z, T = z.double().round() * 4, 1.0
+    if offset == "cold":
+        z, far, T = z * 1e4, z * 1e4, 1e-3
+    else:
+        far = z + offset if abs(offset) < 1e17 else torch.full_like(z, offset)
+        z = z if abs(offset) < 1e17 else torch.zeros_like(z)
+    want = torch.softmax(z / T, 1) * T - torch.zeros_like(z).scatter_add_(1, idx, torch.softmax(t.double() / T, 1)) * T
+    got = oracle.distill(far, t, idx, T, bits=torch.float32, centred=True)
+    assert float((got["dlogits"] - want).abs().max()) < 1e-14
+    assert bool(got["dlogits_off"].isfinite().all()) and float(got["dlogits_off"].max()) < 1e-3
