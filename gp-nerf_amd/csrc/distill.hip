@@ -95,6 +95,12 @@ __device__ __forceinline__ void merge(float& m, float& l, float m2, float l2, fl
   m = M;
 }
 
+// Backward: whether a row's probabilities are formed from its stored log-sum-exp (given in powers of two).  Up to 32 of them half a
+// step of fp32 is 2^-20, about what the row's sum is off by itself; beyond, a common offset of the logits would drown their
+// differences, and the row's maximum and sum are formed once more (4096 x 48000 bf16: 184 us where every row is such a one, 175 where
+// none is; 500 x 140000 bf16, read a second time for it: 83 and 54).
+__device__ __forceinline__ bool lse_serves(float l2) { return fabsf(l2) <= 32.f; }
+
 // log sum exp(z / T) from the maximum and log2 of the sum relative to it.  (m c alone would overflow for logits near the type's
 // limits, whose log-sum-exp is a number.)
 __device__ __forceinline__ float row_lse(const DistP& a, float m, float l2) { return m / a.T + l2 * LN2; }
@@ -161,9 +167,27 @@ __global__ void __launch_bounds__(NT, CH > 8 ? 4 : 6) k_distill_rows(const DistP
   }
 
   // log2 of a logit's probability: (x - m) c - l2.  The difference comes first: x c - m c of logits of 10^9 would be noise.
+  float l2 = MODE == BWD ? a.lse_in[row] * LOG2E : 0.f;
+  const bool walk = MODE != BWD || !lse_serves(l2);
   float m = xe, l = fabsf(xe) == INFINITY ? exp2_(xe) : edge >= 0 ? exp2_((xe - base_of(xe)) * a.c) : 0.f;
-  if (MODE != BWD) {
-    for (int c0 = 0;;) {
+  if (walk) {
+    if constexpr (MANY && MODE == BWD) {
+      // The first segment stays in its registers: a chunk at a time, so that no more of them are taken than for the gradient alone
+      // and two workgroups fit a CU (500 x 140000 bf16, rows whose stored value serves: 54 us, 59 with the loop below).
+#pragma unroll 1
+      for (int c = tid; c < nch; c += NT) {
+        const u4v y = *(const u4v*)((const char*)zc + (unsigned)c * 16u);
+        float mx = m;
+#pragma unroll
+        for (int e = 0; e < EP; ++e) mx = fmaxf(mx, E::get(y, e));
+        const float b = base_of(mx);
+        l *= exp2_((m - b) * a.c);
+        m = mx;
+#pragma unroll
+        for (int e = 0; e < EP; ++e) l += exp2_((E::get(y, e) - b) * a.c);
+      }
+    }
+    for (int c0 = 0; !(MANY && MODE == BWD);) {
       float mx = m;
 #pragma unroll
       for (int i = 0; i < CH; ++i)
@@ -190,18 +214,18 @@ __global__ void __launch_bounds__(NT, CH > 8 ? 4 : 6) k_distill_rows(const DistP
     if (lane == 0) sred[wave] = m, sred[NW + wave] = l;
   }
   __syncthreads();
-  if (MODE != BWD) {
+  if (walk) {
     m = sred[0], l = sred[NW];
 #pragma unroll
     for (int w = 1; w < NW; ++w) merge(m, l, sred[w], sred[NW + w], a.c);
+    l2 = log2_(l);
+  } else {
+    m = 0.f;
   }
   const float mt = sstat[0], lt = sstat[1];
   const float wt = a.w ? a.w[row] : 1.f;
   const bool empty = wt == 0.f || (!(lt > 0.f) && lt == lt);  // left out, or no entry at all
   const float lt2 = log2_(lt);
-  float l2;
-  if (MODE == BWD) m = 0.f, l2 = a.lse_in[row] * LOG2E;
-  else l2 = log2_(l);
   if (MODE != BWD && wave == 0) {
     float loss = 0.f;
     for (int k = lane; k < a.K; k += 64) {
@@ -336,7 +360,14 @@ __global__ void __launch_bounds__(256) k_distill_planes(const DistP a) {
           zl[v * KM + k] = c >= 0 ? E::load(z + v + c * a.z_cs) : 0.f;
         }
     }
-    if (MODE != BWD) {
+    float l2[VEC];
+    bool walk = MODE != BWD;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      l2[v] = MODE == BWD ? a.lse_in[first + v] * LOG2E : 0.f;
+      walk |= MODE == BWD && !lse_serves(l2[v]);
+    }
+    if (walk) {
       if constexpr (CM > 0) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
@@ -366,7 +397,7 @@ __global__ void __launch_bounds__(256) k_distill_planes(const DistP a) {
         }
       }
     }
-    float l2[VEC], mt[VEC], lt2[VEC], f[VEC], fi[VEC];
+    float mt[VEC], lt2[VEC], f[VEC], fi[VEC];
     bool empty[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
@@ -390,7 +421,7 @@ __global__ void __launch_bounds__(256) k_distill_planes(const DistP a) {
       const float wt = a.w ? a.w[row] : 1.f;
       empty[v] = wt == 0.f || (!(lt > 0.f) && lt == lt);  // left out, or no entry at all
       lt2[v] = log2_(lt);
-      if (MODE == BWD) m[v] = 0.f, l2[v] = a.lse_in[row] * LOG2E;
+      if (MODE == BWD && lse_serves(l2[v])) m[v] = 0.f;
       else l2[v] = log2_(l[v]);
       if (MODE != BWD) {
         float loss = 0.f;

@@ -427,3 +427,34 @@ def test_oracle_does_not_depend_on_a_common_offset(offset):
     got = oracle.distill(far, t, idx, T, bits=torch.float32, centred=True)
     assert float((got["dlogits"] - want).abs().max()) < 1e-14
     assert bool(got["dlogits_off"].isfinite().all()) and float(got["dlogits_off"].max()) < 1e-3
+
+
+def _far(kind, dtype, z):
+    """Logits whose common offset, or whose temperature, makes 32 bits of their log-sum-exp too few. -> logits, temperature"""
+    top = torch.finfo(TYPES[dtype]).max
+    if kind == "cold":
+        return z * 10.0, 1e-3
+    if kind == "lowest":
+        return torch.full_like(z, -top), 1.0
+    return (z.float() + kind).to(z.dtype), 1.0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("kind", [30.0, -1e5, 1e7, -1e9, "cold", "lowest"], ids=str)
+@pytest.mark.parametrize("planes,N,C,K", [(False, 9, 60, 5), (False, 5, 1000, 5), (False, 3, 9001, 5), (False, 2, 140000, 5),
+                                          (True, 60, 21, 5), (True, 61, 21, 12), (True, 60, 70, 5), (True, 31, 70, 12)])
+def test_offsets_that_cancel_in_the_softmax(dtype, kind, planes, N, C, K):
+    """Forward and backward apart against the formula (as exact as the step, whose logits are taken relative to the maximum)."""
+    from gp_nerf_amd import semantic_branch as S
+    z, t, idx = _inputs(dtype, N, C, K, planes=planes)
+    far, T = _far(kind, dtype, z)
+    z = torch.where(torch.arange(N, device="cuda")[:, None] % 3 == 1, z, far)   # ordinary rows beside them
+    if planes:
+        z = z.t().contiguous().t()
+    want = oracle.distill(z, t, idx, T, bits=z.dtype, centred=True)
+    assert bool(want["dlogits_off"].isfinite().all())
+    loss, lse = S.distill_topk_forward(z, t, idx, T, None, "none")
+    _near("lse", lse, want)
+    _near("dlogits", S.distill_topk_backward(torch.ones(N, device="cuda"), z, t, idx, lse, T, None, "none"), want)
+    _near("dlogits", S.distill_topk_step(z, t, idx, T, None, "none")[1], want)
