@@ -139,8 +139,8 @@ def attention_backward(dout, q, k, v, out, lse, lengths=None, key_mask=None, cau
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, lengths, key_mask, causal, q_start, scale):
-        if any(ctx.needs_input_grad):
+    def forward(ctx, q, k, v, lengths, key_mask, causal, q_start, scale, recording):
+        if recording and any(ctx.needs_input_grad):  # (which says what the arguments require, under no_grad too)
             _lib.refuse_capture("attention", "attention_forward and attention_backward")
         out, lse = attention_forward(q, k, v, lengths, key_mask, causal, q_start, scale)
         ctx.save_for_backward(q, k, v, out, lse, lengths, key_mask, q_start)
@@ -153,9 +153,9 @@ class _Attention(torch.autograd.Function):
         _lib.refuse_capture("attention", "attention_forward and attention_backward")
         q, k, v, out, lse, lengths, key_mask, q_start = ctx.saved_tensors
         grads = attention_backward(dout, q, k, v, out, lse, lengths, key_mask, ctx.causal, q_start, ctx.scale)
-        return (*grads, None, None, None, None, None)
+        return (*grads, None, None, None, None, None, None)
 
 
 def attention(q, k, v, lengths=None, key_mask=None, causal=False, q_start=None, scale=None):
-    """attention_forward's output, differentiable in q, k and v (once; not inside a captured graph)."""
-    return _Attention.apply(q, k, v, lengths, key_mask, causal, q_start, scale)
+    """attention_forward's output, differentiable in q, k and v (once; not inside a captured graph, unless under no_grad)."""
+    return _Attention.apply(q, k, v, lengths, key_mask, causal, q_start, scale, torch.is_grad_enabled())

@@ -160,8 +160,8 @@ def distill_topk_step(logits, teacher_logits, teacher_index, temperature=1.0, ro
 
 class _DistillTopK(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, teacher_logits, teacher_index, temperature, row_weight, reduction):
-        if ctx.needs_input_grad[0]:
+    def forward(ctx, logits, teacher_logits, teacher_index, temperature, row_weight, reduction, recording):
+        if recording and ctx.needs_input_grad[0]:  # (which says what the logits require, under no_grad too)
             _lib.refuse_capture("distill_topk_loss", "distill_topk_step")
         loss, lse = distill_topk_forward(logits, teacher_logits, teacher_index, temperature, row_weight, reduction)
         ctx.save_for_backward(logits, teacher_logits, teacher_index, row_weight, lse)
@@ -173,13 +173,14 @@ class _DistillTopK(torch.autograd.Function):
     def backward(ctx, dloss):
         _lib.refuse_capture("distill_topk_loss", "distill_topk_step")
         logits, t, x, w, lse = ctx.saved_tensors
-        return (distill_topk_backward(dloss, logits, t, x, lse, ctx.temperature, w, ctx.reduction), None, None, None, None, None)
+        return (distill_topk_backward(dloss, logits, t, x, lse, ctx.temperature, w, ctx.reduction), None, None, None, None, None,
+                None)
 
 
 def distill_topk_loss(logits, teacher_logits, teacher_index, temperature=1.0, row_weight=None, reduction="mean"):
-    """distill_topk_forward's loss, differentiable in the logits (once; not inside a captured graph).  The teacher and the
-    weights take no gradient."""
-    return _DistillTopK.apply(logits, teacher_logits, teacher_index, temperature, row_weight, reduction)
+    """distill_topk_forward's loss, differentiable in the logits (once; not inside a captured graph, unless under no_grad).  The
+    teacher and the weights take no gradient."""
+    return _DistillTopK.apply(logits, teacher_logits, teacher_index, temperature, row_weight, reduction, torch.is_grad_enabled())
 
 
 class _ConvGNReLU(nn.Conv2d):

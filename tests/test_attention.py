@@ -644,3 +644,35 @@ def test_gradients_of_hidden_keys_are_zero_under_overflown_ones(dtype, shape):
     q[1, 1, 1, 5] = float("nan")
     got = _both(q, k, v, do, lengths=lengths, key_mask=mask)
     assert not bool(got["dk"][hide].any()) and not bool(got["dv"][hide].any())
+
+
+@pytest.mark.parametrize("recording", [True, False])
+def test_capture_is_refused_for_recorded_graphs_only(monkeypatch, recording):
+    """Nothing is recorded under no_grad, whatever the arguments require: the refusal there is the one of CPU tensors."""
+    from gp_nerf_amd.attention import attention
+    q, k, v, _ = _inputs("fp32", 1, 2, 3, 2, 1, 16, dev="cpu")
+    k.requires_grad_(True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with torch.set_grad_enabled(recording), pytest.raises(RuntimeError, match="cannot be captured" if recording else "no CPU fallback"):
+        attention(q, k, v)
+
+
+@pytest.mark.gpu
+def test_captured_without_a_graph():
+    """The differentiable form of leaves that require gradients, captured under no_grad."""
+    from gp_nerf_amd.attention import attention, attention_forward
+    q, k, v, _ = _inputs("bf16", 2, 50, 70, 4, 2, 32)
+    leaf = q.clone().requires_grad_(True)
+    attention_forward(q, k, v)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g), torch.no_grad():
+        out = attention(leaf, k, v)
+    for seed in (1, 2, 3):
+        new = _inputs("bf16", 2, 50, 70, 4, 2, 32, seed=seed)[0]
+        with torch.no_grad():
+            leaf.copy_(new)
+        g.replay()
+        want = attention_forward(new, k, v)[0]
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)

@@ -458,3 +458,34 @@ def test_offsets_that_cancel_in_the_softmax(dtype, kind, planes, N, C, K):
     _near("lse", lse, want)
     _near("dlogits", S.distill_topk_backward(torch.ones(N, device="cuda"), z, t, idx, lse, T, None, "none"), want)
     _near("dlogits", S.distill_topk_step(z, t, idx, T, None, "none")[1], want)
+
+
+@pytest.mark.parametrize("recording", [True, False])
+def test_capture_is_refused_for_recorded_graphs_only(monkeypatch, recording):
+    """Nothing is recorded under no_grad, whatever the logits require: the refusal there is the one of CPU tensors."""
+    from gp_nerf_amd import semantic_branch as S
+    z, t, idx = _inputs("fp32", 4, 6, 2, dev="cpu")
+    z.requires_grad_(True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with torch.set_grad_enabled(recording), pytest.raises(RuntimeError, match="cannot be captured" if recording else "no CPU fallback"):
+        S.distill_topk_loss(z, t, idx)
+
+
+@pytest.mark.gpu
+def test_captured_loss_without_a_graph():
+    from gp_nerf_amd import semantic_branch as S
+    z, t, idx = _inputs("fp32", 33, 700, 5)
+    leaf = z.clone().requires_grad_(True)
+    S.distill_topk_forward(z, t, idx)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g), torch.no_grad():
+        loss = S.distill_topk_loss(leaf, t, idx)
+    for seed in (1, 2, 3):
+        new = _inputs("fp32", 33, 700, 5, seed=seed)[0]
+        with torch.no_grad():
+            leaf.copy_(new)
+        g.replay()
+        want = S.distill_topk_forward(new, t, idx)[0]
+        torch.cuda.synchronize()
+        assert torch.equal(loss, want)
