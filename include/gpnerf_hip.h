@@ -416,7 +416,8 @@ typedef struct {
   size_t workspace_bytes;
 } gpn_attn_args_t;
 
-/* Depends on the sizes alone; 0 for sizes that gpn_attn_forward / gpn_attn_backward refuse. */
+/* Ask with the arguments of the call: with `backward` it depends on the strides beside the sizes (short sequences need none unless
+ * their positions or heads lie 2^20 elements apart or more).  0 for sizes that gpn_attn_forward / gpn_attn_backward refuse. */
 size_t gpn_attn_workspace_bytes(const gpn_attn_args_t* a, int backward);
 int gpn_attn_forward(const gpn_attn_args_t* a, gpn_stream_t stream);
 /* dq, dk, dv of sum(out * dout): the probabilities are computed again from q, k and lse. */
