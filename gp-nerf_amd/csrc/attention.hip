@@ -663,8 +663,8 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_one_piece(const AttnP a) {
 
 // Few rows (new tokens of sequences, or too few tiles to fill the card): the WK waves share a tile of rows and divide the keys,
 // each with stages of its own and no barrier until their sums are joined.
-// Bound by memory for long keys: one query for each of 8 sequences of 16 K keys, 32 heads on 8 of 128, bf16: 109 us, 4.9 TB/s; with
-// lengths from 0 to 16 K 74 us.  One query against 257 keys: 7 us, the latency of three loads in a row.
+// Bound by memory for long keys: one query for each of 8 sequences of 16 K keys, 32 heads on 8 of 128, bf16: 107 us, 5.0 TB/s; fp32:
+// 202 us, 5.3 TB/s; with lengths from 0 to 16 K 74 us in bf16.  One query against 257 keys: 7 us, the latency of three loads in a row.
 template <typename T, int DP, int WK, int KT>
 struct Few {
   using L = Lay<T, DP>;
@@ -696,7 +696,8 @@ __global__ void __launch_bounds__(64 * WK, 2) k_attn_few(const AttnP a) {
     load_keys<T, DP, KT, 1>(kb, a.sk.l, a.D, j0, bits, base + buf * 2 * F::TILE, 0, lane);
     load_keys<T, DP, KT, 1>(vb, a.sv.l, a.D, j0, bits, base + (buf * 2 + 1) * F::TILE, 0, lane);
   };
-  // two stages on their way: the second lands while the first is worked on, whose memory the third then takes
+  // two stages on their way: the second lands while the first is worked on, whose memory the third then takes.  With a key mask one:
+  // the compiler, which does not count these loads, waits for all of them where it waits for the mask's bytes.
   constexpr int NEXT = WK * KT, LOADS = 2 * Dma<T, DP, KT, 1>::COUNT;
   const int jb = r.kbeg + wave * KT;
   keys.fetch(jb, lane);
@@ -943,7 +944,8 @@ __global__ void __launch_bounds__(64 * NW * WK, 2) k_attn_dq(const AttnP a) {
 // Keys and values are stationary, a wave holds TM of them; the rows of all query heads that share them walk past, so the sum
 // over the group is part of the walk and its order is fixed.  WN waves along the keys x WR waves along the rows: the WR waves of
 // the same keys take the rows of a stage in turns and join their sums at the end, so that two waves fit a SIMD (256 registers)
-// without a second copy of the keys' sums in memory.  Where those registers are short (VL) the values come from LDS.
+// without a second copy of the keys' sums in memory.  Where those registers are short (VL) the values come from LDS; pairs of
+// 128-wide bf16 heads still lack three, which lie in scratch.
 // Work is cut evenly: under `causal` a workgroup takes the key tiles t and tiles - 1 - t, which together see as many rows as any
 // other such pair, and every tile's own rows are cut into nsplit parts (fp32 sums in the workspace, joined in order).
 // Bound by LDS as well: every row is read from there twice in each direction, for four products.  4 x 4096, 16 heads of 64, bf16:
@@ -1454,7 +1456,7 @@ Plan plan_forward(const gpn_attn_args_t* x) {
                      prob * ((M + small - 1) / small) >= 256;
   p.few = M <= small || steep;
   // wide fp32 heads, of which such a wave takes 16 keys at a time: only where tiles of many rows leave no room for parts of the keys
-  // (333 x 6 heads of 80, 1021 keys: 41 against 43 us)
+  // (3 x 333, 6 query and 3 key/value heads, 1021 keys: of 80 40 against 43 us, of 128 54 against 58)
   p.mid = !p.few && is_mid(prob, M, f32, x->D, x->causal) && !(f32 && x->D > 64 && large <= 128);
   p.bm = p.few ? small : p.mid ? big / 2 : big;
   p.tiles = (int)((M + p.bm - 1) / p.bm);
@@ -1462,7 +1464,8 @@ Plan plan_forward(const gpn_attn_args_t* x) {
   // min_part or more so that a part outweighs its share of the join.  (One query, 8 heads, 64 K keys: 64 parts 51 us, 5.3 TB/s;
   // twice as many workgroups for eight queries of uneven lengths 82 against 76 us.)  Workgroups of many rows that are more than
   // half the CUs' number only where the keys are long or their products slow (1100 queries, 16 K keys, 8 heads of 128: 240 us in
-  // one part, 130 in two; fp32 2 x 400, 4 x 2 heads of 128, 1400 keys: 93 and 73; but 2 x 777, 8 query and 2 key/value heads of 64: 16, 21).
+  // one part, 130 in three; fp32 2 x 400, 8 query and 4 key/value heads of 128, 1400 keys: 132 and 70; but 2 x 777, 8 query and 2
+  // key/value heads of 64: 16, 21).
   const long long units = prob * p.tiles, min_part = f32 ? 128 : 256;
   const long long split_to = M <= small ? 512 : steep ? 0 : (f32 && x->D > 64) || x->Lk >= 2048 ? 256 : 128;
   const long long s = units < 1 || units > split_to ? 1 : std::min({512 / units, x->Lk / min_part, (long long)MAX_SPLIT});
