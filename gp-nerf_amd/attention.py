@@ -9,8 +9,8 @@ not cover: training, longer sequences, masks, shared key/value heads, and single
     out = attention(q, k, v)                                  the same pair behind torch.autograd
 
 q is [B, Lq, Hq, D]; k and v are [B, Lk, Hkv, D]; query head h reads key/value head h // (Hq // Hkv).  float32 or bfloat16, all
-of one type; D a multiple of 8 up to 128.  Any strides (slices of a cache, expanded tensors); a tensor whose last dimension is
-not contiguous or whose rows are not 16-byte aligned is copied first.
+of one type; D a multiple of 8 up to 128; Hq at most 256 Hkv, Lq * Hq / Hkv and B * Hkv at most 2^24.  Any strides (slices of a
+cache, expanded tensors); a tensor whose last dimension is not contiguous or whose rows are not 16-byte aligned is copied first.
 
 A key is visible to a query where all of these hold:
     lengths   [B] int32: the key's position is below its batch's length

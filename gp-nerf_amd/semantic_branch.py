@@ -117,9 +117,9 @@ def distill_topk_forward(logits, teacher_logits, teacher_index, temperature=1.0,
     temperature T || softmax of all the student's classes at T).
 
     logits [N, C] (any strides with contiguous classes or contiguous rows, others are copied; with contiguous classes at most
-    4194303 rows) or an image [1, C, H, W] as NeRFSemSegFPNHead gives it; float32 or bfloat16.  teacher_logits, teacher_index [N, K] (or [1, K, H, W]): what
-    `teacher.topk(K, dim=1)` returns; int32 or int64 classes; an entry outside [0, C) (-1) is left out and a row
-    without an entry counts as zero.  row_weight [N] float32: weight of each row (0 leaves it out, whatever it holds).
+    4194303 rows) or an image [1, C, H, W] as NeRFSemSegFPNHead gives it; float32 or bfloat16.  teacher_logits, teacher_index
+    [N, K] (or [1, K, H, W]): what `teacher.topk(K, dim=1)` returns; int32 or int64 classes; an entry outside [0, C) (-1) is left
+    out and a row without an entry counts as zero.  row_weight [N] float32: weight of each row (0 leaves it out, whatever it holds).
     reduction: 'mean' over all N rows, 'sum' or 'none'.  temperature from 1e-12 to 1e12.  -> loss (scalar, or [N]), lse [N]
     (what distill_topk_backward needs).  No graph is recorded."""
     head, z, _, keep = _distill_args(logits, teacher_logits, teacher_index, temperature, row_weight, reduction)

@@ -397,7 +397,8 @@ int gpn_gnt_forward_static(const gpn_gnt_weights_t* W, const float* rgb_feat, in
 
 typedef struct {
   int dtype;                 /* GPN_DT_*: of q, k, v, out, dout, dq, dk, dv */
-  int B, Lq, Lk, Hq, Hkv, D; /* Hq a multiple of Hkv; D a multiple of 8, at most GPN_ATTN_MAX_D */
+  int B, Lq, Lk, Hq, Hkv, D; /* Hq a multiple of Hkv, at most 256 times it; D a multiple of 8, at most GPN_ATTN_MAX_D;
+                                Lq * Hq / Hkv and B * Hkv at most 2^24, Lk at most 2^30 */
   int causal;
   float scale;               /* 1e-30 to 1e30 */
   const void *q, *k, *v;     /* [B,Lq,Hq,D], [B,Lk,Hkv,D] x 2: 16-byte aligned, contiguous along D, and strided: */
